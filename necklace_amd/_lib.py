@@ -8,6 +8,8 @@ is raised.  Nothing here computes on the CPU.
 sum over interleaved payloads.  The package never loads it by itself; sweeps and
 tests that want it either call it directly or make it the bound library for a
 while with `use_tuning_library()`.
+
+`mx_lib()` binds libnkmx.so, the microscaled operators (include/nkmx.h).
 """
 import contextlib
 import ctypes as ct
@@ -22,6 +24,7 @@ import torch  # noqa: F401
 _PKG = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(_PKG, "libnklq.so")
 TUNING_SO_PATH = os.path.join(_PKG, "libnklq_tuning.so")
+MX_SO_PATH = os.path.join(_PKG, "libnkmx.so")
 
 NKLQ_MAX_PAYLOADS_PER_LAUNCH = 16
 
@@ -32,13 +35,26 @@ SYMBOLS = (
 )
 TUNING_SYMBOLS = ("nklq_copy_f32", "nklq_tuning_sum_interleaved_f32")
 
+MX_SYMBOLS = (
+    "nkmx_mx4_quantize", "nkmx_mx4_dequantize", "nkmx_mx4_matmul", "nkmx_mx4_linear", "nkmx_mx4_linear_workspace",
+    "nkmx_act8_save", "nkmx_act8_load", "nkmx_act8_grad", "nkmx_act8_wgrad", "nkmx_act8_wgrad_workspace",
+    "nkmx_strerror", "nkmx_version",
+)
+
 _lib = None
 _tuning = None
+_mx = None
 
 
 class NklqError(RuntimeError):
     def __init__(self, code, text):
         super().__init__(f"libnklq error {code}: {text}")
+        self.code = code
+
+
+class NkmxError(RuntimeError):
+    def __init__(self, code, text):
+        super().__init__(f"libnkmx error {code}: {text}")
         self.code = code
 
 
@@ -96,6 +112,44 @@ def tuning_lib():
             f"{TUNING_SO_PATH} is missing: build it with `python -m necklace_amd.csrc.build --tuning`")
     _tuning = _bind(TUNING_SO_PATH, tuning=True)
     return _tuning
+
+
+def mx_lib():
+    """The library of the microscaled operators; raises if it has not been built."""
+    global _mx
+    if _mx is not None:
+        return _mx
+    if not os.path.exists(MX_SO_PATH):
+        raise ImportError(
+            f"{MX_SO_PATH} is missing: build it with `python -m necklace_amd.csrc.build` "
+            "(needs hipcc; there is no CPU fallback)")
+    L = ct.CDLL(MX_SO_PATH)
+    vp, u64, i32 = ct.c_void_p, ct.c_uint64, ct.c_int
+    for name, args in {
+            "nkmx_mx4_quantize": [vp, i32, u64, u64, u64, vp, vp, i32, vp],
+            "nkmx_mx4_dequantize": [vp, i32, u64, u64, u64, vp, vp, vp],
+            "nkmx_mx4_matmul": [vp, i32, u64, u64, u64, u64, vp, vp, vp, vp, vp, vp],
+            "nkmx_mx4_linear": [vp, vp, i32, u64, u64, u64, u64, u64, vp, vp, vp, vp, u64, vp],
+            "nkmx_act8_save": [vp, vp, i32, i32, u64, u64, u64, u64, vp, vp, vp],
+            "nkmx_act8_load": [vp, i32, u64, u64, u64, vp, vp, vp],
+            "nkmx_act8_grad": [vp, vp, i32, i32, u64, u64, u64, u64, vp, vp, vp],
+            "nkmx_act8_wgrad": [vp, vp, vp, i32, u64, u64, u64, u64, u64, vp, vp, i32, vp, u64, vp],
+            "nkmx_strerror": [i32],
+            "nkmx_version": []}.items():
+        getattr(L, name).argtypes = args
+        getattr(L, name).restype = i32
+    L.nkmx_strerror.restype = ct.c_char_p
+    L.nkmx_mx4_linear_workspace.argtypes = [u64, u64, u64]
+    L.nkmx_mx4_linear_workspace.restype = u64
+    L.nkmx_act8_wgrad_workspace.argtypes = [i32, u64, u64, u64]
+    L.nkmx_act8_wgrad_workspace.restype = u64
+    _mx = L
+    return _mx
+
+
+def check_mx(code):
+    if code != 0:
+        raise NkmxError(code, mx_lib().nkmx_strerror(code).decode())
 
 
 @contextlib.contextmanager

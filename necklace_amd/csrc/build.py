@@ -1,11 +1,12 @@
-"""Compiles csrc/nklq.hip for gfx950 (MI355X).
+"""Compiles csrc/nklq.hip and csrc/nkmx.hip for gfx950 (MI355X).
 
-    python -m necklace_amd.csrc.build            # necklace_amd/libnklq.so, the product library
+    python -m necklace_amd.csrc.build            # necklace_amd/libnklq.so and libnkmx.so, the product libraries
     python -m necklace_amd.csrc.build --tuning   # necklace_amd/libnklq_tuning.so as well
 
 The tuning library is the same source with -DNKLQ_TUNING_BUILD=1: every launch geometry nklq_tune
 can name, a copy kernel and the sum over interleaved payloads (include/nklq_tuning.h).  Only the
-geometry sweeps of bench.py and the parity tests that run every geometry load it.
+geometry sweeps of bench.py and the parity tests that run every geometry load it.  libnkmx.so holds
+the microscaled operators (include/nkmx.h).
 
 hipcc cross-compiles without a GPU present.  The libraries are kept inside the
 package directory so that they are found next to the Python sources.
@@ -19,6 +20,7 @@ PKG = os.path.dirname(CSRC)
 ROOT = os.path.dirname(PKG)
 SO_PATH = os.path.join(PKG, "libnklq.so")
 TUNING_SO_PATH = os.path.join(PKG, "libnklq_tuning.so")
+MX_SO_PATH = os.path.join(PKG, "libnkmx.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -32,10 +34,18 @@ FLAGS = [
 
 
 def build(verbose=False, tuning=False):
-    """Compile the product library, or with tuning=True the measurement build of the same source."""
-    target = TUNING_SO_PATH if tuning else SO_PATH
-    cmd = [HIPCC, *FLAGS, *(["-DNKLQ_TUNING_BUILD=1"] if tuning else []), "-I", os.path.join(ROOT, "include"),
-           os.path.join(CSRC, "nklq.hip"), "-o", target]
+    """Compile the quantizer's product library, or with tuning=True the measurement build of the same source."""
+    return _compile("nklq.hip", TUNING_SO_PATH if tuning else SO_PATH,
+                    ["-DNKLQ_TUNING_BUILD=1"] if tuning else [], verbose)
+
+
+def build_mx(verbose=False):
+    """Compile the library of the microscaled operators."""
+    return _compile("nkmx.hip", MX_SO_PATH, [], verbose)
+
+
+def _compile(source, target, extra, verbose):
+    cmd = [HIPCC, *FLAGS, *extra, "-I", os.path.join(ROOT, "include"), os.path.join(CSRC, source), "-o", target]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
@@ -50,14 +60,17 @@ def build(verbose=False, tuning=False):
 
 
 def ensure_built(tuning=False):
-    """Build only when no library is there yet (a fresh checkout: the .so is not in version control)."""
+    """Build only what is not there yet (a fresh checkout: the .so files are not in version control)."""
     target = TUNING_SO_PATH if tuning else SO_PATH
     if not os.path.exists(target):
         build(tuning=tuning)
+    if not os.path.exists(MX_SO_PATH):
+        build_mx()
     return target
 
 
 if __name__ == "__main__":
     print(build(verbose="-q" not in sys.argv))
+    print(build_mx(verbose="-q" not in sys.argv))
     if "--tuning" in sys.argv:
         print(build(verbose="-q" not in sys.argv, tuning=True))

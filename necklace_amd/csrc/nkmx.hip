@@ -1,0 +1,1415 @@
+// nkmx.hip — microscaled storage for MI355X (gfx950, CDNA4): 4-bit floating point with its products,
+// and 8-bit activation checkpoints with the gradients that read them (include/nkmx.h has the formats).
+//
+// Two kinds of kernel:
+//   * streaming passes (quantize, save, load, gradient of the activation): bound by HBM.  A lane moves 16
+//     bytes of numbers per request, a block of 32 columns is 4 or 8 neighbouring lanes, and its largest
+//     magnitude travels between them in DPP moves; codes and scales leave in whole contiguous runs;
+//   * products: matrix instructions over tiles in LDS.  mx4 operands go to the scaled matrix instruction
+//     as they are stored; an 8-bit checkpoint is turned into bf16 on its way into LDS, which is exact
+//     (7 bits of magnitude times a power of two).
+//
+// fp32 arithmetic is IEEE: no fast-math, no contraction, denormals kept.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <tuple>
+#include <type_traits>
+#include <utility>
+
+#include "nkmx.h"
+
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kStep = NKMX_STEP;        // columns of a step
+constexpr int kStepBytes4 = kStep / 2;  // its mx4 codes
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// n / d for 32-bit n: one high product with a 64-bit reciprocal (exact: the error of the reciprocal, below
+// 2^-64 relative to 1/d, times n < 2^32 stays below 1/d).
+struct FastDiv {
+    uint64_t inv;  // floor(2^64 / d) + 1, 0 for d = 1
+    uint32_t d;
+};
+inline FastDiv fast_div(uint32_t d) { return FastDiv{d > 1 ? ~0ull / d + 1 : 0, d}; }
+__device__ __forceinline__ uint32_t quotient(uint32_t n, FastDiv f)
+{
+    return f.inv ? (uint32_t)__umul64hi((uint64_t)n, f.inv) : n;
+}
+
+// ---------------------------------------------------------------- numbers
+
+template <typename T>
+__device__ __forceinline__ float number(T v) { return (float)v; }
+
+// Magnitude bits of an fp32 value: ordered like the magnitudes, infinity and NaN above every number.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// The scale byte of a block from its largest magnitude: the exponent byte of that number less TOP (2 for
+// codes up to 6, 6 for codes up to 127), held at 0 = 2^-127; subnormal magnitudes (exponent byte 0) are below
+// every scale and get 0 as well.
+template <int TOP>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top)
+{
+    const uint32_t e = top >> 23;
+    return e == 255u ? 255u : (e > (uint32_t)TOP ? e - TOP : 0u);
+}
+
+// 2^(byte - 127) for bytes below 255 (2^-127 is a subnormal fp32 number); NaN for 255.
+__device__ __forceinline__ float scale_value(uint32_t byte)
+{
+    const uint32_t bits = byte == 0u ? 0x00400000u : byte << 23;
+    return __uint_as_float(byte == 255u ? 0x7FC00000u : bits);
+}
+// 2^(127 - byte) for bytes up to 253 (a finite number's byte is 252 at most).
+__device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+// Phi(x) = erfc(-x / sqrt 2) / 2 with Abramowitz and Stegun's formula 7.1.26, erfc(z) = (a1 t + .. + a5 t^5)
+// e^(-z^2), t = 1 / (1 + p z) for z >= 0, |error| <= 1.5e-7; `tail` gets e^(-x^2 / 2).
+__device__ __forceinline__ float normal_distribution(float x, float& tail)
+{
+    const float z = fabsf(x) * 0.70710678118654752f;
+    tail = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float half = 0.5f * (p * t * tail);
+    return x < 0.0f ? half : 1.0f - half;
+}
+
+__device__ __forceinline__ float logistic(float x)
+{
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+}
+
+template <int FN>
+__device__ __forceinline__ float activation(float x)
+{
+    if constexpr (FN == NKMX_GELU) {
+        float tail;
+        return x * normal_distribution(x, tail);
+    } else if constexpr (FN == NKMX_SILU) {
+        return x * logistic(x);
+    }
+    return x;
+}
+
+template <int FN>
+__device__ __forceinline__ float activation_slope(float x)
+{
+    if constexpr (FN == NKMX_GELU) {
+        float tail;
+        const float phi = normal_distribution(x, tail);
+        return fmaf(x * 0.39894228040143268f, tail, phi);
+    } else if constexpr (FN == NKMX_SILU) {
+        const float s = logistic(x);
+        return s * fmaf(x, 1.0f - s, 1.0f);
+    }
+    return 1.0f;
+}
+
+// ---------------------------------------------------------------- lane exchange
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
+constexpr int kQuadSwap1 = 0xB1, kQuadSwap2 = 0x4E, kHalfMirror = 0x141, kRowRor4 = 0x124, kRowRor8 = 0x128;
+
+// Largest value over the lanes that share a block: 4 lanes of 8 elements or 8 lanes of 4.
+template <int LANES>
+__device__ __forceinline__ uint32_t block_max(uint32_t v)
+{
+    v = max(v, dpp<kQuadSwap1>(v));
+    v = max(v, dpp<kQuadSwap2>(v));
+    if constexpr (LANES == 8) v = max(v, dpp<kHalfMirror>(v));
+    return v;
+}
+
+// The scale bytes of a DPP row's blocks (4 or 2 of them) side by side, in every lane of the row.
+template <int LANES>
+__device__ __forceinline__ uint32_t row_scales(uint32_t byte, int lane)
+{
+    uint32_t v = byte << (8 * ((lane & 15) / LANES));
+    if constexpr (LANES == 4) v |= dpp<kRowRor4>(v);
+    return v | dpp<kRowRor8>(v);
+}
+
+// ---------------------------------------------------------------- memory access
+
+// E neighbouring elements; only the alignment of the type is promised (views start anywhere).
+template <typename T, int E>
+struct Pack {
+    typedef T vec __attribute__((ext_vector_type(E)));
+    typedef vec loose __attribute__((aligned(sizeof(T))));
+};
+
+template <typename T, int E>
+__device__ __forceinline__ typename Pack<T, E>::vec load_pack(const T* p, int64_t live)
+{
+    typedef typename Pack<T, E>::vec V;
+    typedef typename Pack<T, E>::loose L;
+    V v;
+    if (live >= E) {
+        v = __builtin_nontemporal_load(reinterpret_cast<const L*>(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = i < live ? p[i] : (T)0.0f;
+    }
+    return v;
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void store_pack(T* p, typename Pack<T, E>::vec v, int64_t live)
+{
+    typedef typename Pack<T, E>::loose L;
+    if (live >= E) {
+        __builtin_nontemporal_store(v, reinterpret_cast<L*>(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i < live) p[i] = v[i];
+    }
+}
+
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> { typedef uint16_t type; };
+template <>
+struct Word<4> { typedef uint32_t type; };
+template <>
+struct Word<8> { typedef u32x2 type; };
+
+// ---------------------------------------------------------------- streaming passes
+//
+// One lane owns E = 16 bytes / sizeof(T) neighbouring elements; the lanes of a step (128 columns: 16 or 32
+// lanes) lie together, and as packed rows have no gaps, lane i of the launch owns codes i * E onwards: codes
+// and scales are written (read) as one contiguous run whatever the row length is.  Rows and steps come from
+// one division of the step's index.  Workgroups load once, store once and end: the form in which the 2-bit
+// quantizer's kernels stream fastest as well.
+
+template <typename T>
+struct Lanes {
+    static constexpr int E = 16 / (int)sizeof(T);
+    static constexpr int step = kStep / E;             // lanes of a step
+    static constexpr int block = NKMX_BLOCK / E;       // lanes of a block
+    static constexpr int row_blocks = 16 / block;      // blocks of a DPP row
+};
+
+struct Place {
+    uint64_t lane;     // index of the lane in the launch
+    uint32_t row;
+    uint32_t col;
+    int64_t live;      // elements of the matrix from this one on, to the end of the row (<= 0 in the padding)
+};
+
+template <typename T>
+__device__ __forceinline__ bool place_of(Place& p, FastDiv steps, uint32_t n_steps, uint32_t cols)
+{
+    p.lane = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t step = p.lane / Lanes<T>::step;
+    if (step >= n_steps) return false;  // all lanes of a step leave together
+    p.row = quotient((uint32_t)step, steps);
+    p.col = ((uint32_t)step - p.row * steps.d) * kStep + (uint32_t)(p.lane % Lanes<T>::step) * Lanes<T>::E;
+    p.live = (int64_t)cols - (int64_t)p.col;
+    return true;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_scales(uint8_t* scales, const Place& p, uint32_t byte)
+{
+    const uint32_t v = row_scales<Lanes<T>::block>(byte, (int)(p.lane & 63));
+    if ((p.lane & 15) == 0) {
+        typedef typename Word<Lanes<T>::row_blocks>::type W;
+        reinterpret_cast<W*>(scales)[p.lane / 16] = (W)v;
+    }
+}
+
+// Largest magnitude of a lane's elements, as fp32 bits.  16-bit types compare two at a time: their magnitude
+// bits are ordered as whole numbers too.
+__device__ __forceinline__ uint32_t lane_max(Pack<float, 4>::vec v)
+{
+    return max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
+}
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t lane_max_halves(u32x4 w)
+{
+    u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+    return max((uint32_t)m[0], (uint32_t)m[1]);
+}
+__device__ __forceinline__ uint32_t lane_max(Pack<bf16, 8>::vec v)
+{
+    return lane_max_halves(__builtin_bit_cast(u32x4, v)) << 16;
+}
+__device__ __forceinline__ uint32_t lane_max(Pack<f16, 8>::vec v)
+{
+    const uint16_t h = (uint16_t)lane_max_halves(__builtin_bit_cast(u32x4, v));
+    return __float_as_uint((float)__builtin_bit_cast(f16, h));
+}
+
+// mx4 codes of a pair of values, into byte B of `word`.  The convert instruction divides by the scale, rounds
+// to the nearest code with ties to even and saturates (checked against the formula for every kind of tie and
+// scales from 2^-127 up).
+template <int B>
+__device__ __forceinline__ uint32_t pair4(uint32_t word, float a, float b, float scale)
+{
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, a, b, scale, B);
+}
+template <int B>
+__device__ __forceinline__ uint32_t pair4(uint32_t word, bf16 a, bf16 b, float scale)
+{
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, bf16x2{a, b}, scale, B);
+}
+template <int B>
+__device__ __forceinline__ uint32_t pair4(uint32_t word, f16 a, f16 b, float scale)
+{
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, f16x2{a, b}, scale, B);
+}
+
+template <typename V, int N>
+__device__ __forceinline__ uint32_t codes4(V v, float scale)  // N = 4 or 8 values
+{
+    uint32_t w = pair4<0>(0u, v[0], v[1], scale);
+    w = pair4<1>(w, v[2], v[3], scale);
+    if constexpr (N == 8) {
+        w = pair4<2>(w, v[4], v[5], scale);
+        w = pair4<3>(w, v[6], v[7], scale);
+    }
+    return w;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* x, uint64_t ldx, uint8_t* codes, uint8_t* scales,
+                                                           FastDiv steps, uint32_t n_steps, uint32_t cols)
+{
+    constexpr int E = Lanes<T>::E;
+    Place p;
+    if (!place_of<T>(p, steps, n_steps, cols)) return;
+    const auto v = load_pack<T, E>(x + p.row * ldx + p.col, p.live);
+    const uint32_t byte = scale_byte<2>(block_max<Lanes<T>::block>(lane_max(v)));
+    uint32_t w = codes4<decltype(v), E>(v, scale_value(byte));
+    if (byte == 255u) w = 0u;
+    typedef typename Word<E / 2>::type W;
+    reinterpret_cast<W*>(codes)[p.lane] = (W)w;
+    store_scales<T>(scales, p, byte);
+}
+
+// q = x / 2^e to the nearest whole number: adding 1.5 * 2^23 in one rounding leaves it in the low bits, so
+// the byte is cut out of the sum; x * 2^-e is exact inside the fused operation.
+__device__ __forceinline__ uint32_t whole8(float x, float inverse)
+{
+    constexpr float kMagic = 12582912.0f;
+    const float s = fmaf(x, inverse, kMagic);
+    return __float_as_uint(__builtin_amdgcn_fmed3f(s, kMagic - 127.0f, kMagic + 127.0f));
+}
+
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x0C0C0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+    return ab | cd;
+}
+
+template <typename T, int FN>
+__global__ __launch_bounds__(256) void act8_save_kernel(const T* x, uint64_t ldx, T* y, uint64_t ldy, uint8_t* codes,
+                                                        uint8_t* scales, FastDiv steps, uint32_t n_steps, uint32_t cols)
+{
+    constexpr int E = Lanes<T>::E;
+    Place p;
+    if (!place_of<T>(p, steps, n_steps, cols)) return;
+    const auto v = load_pack<T, E>(x + p.row * ldx + p.col, p.live);
+    const uint32_t byte = scale_byte<6>(block_max<Lanes<T>::block>(lane_max(v)));
+    const float inverse = scale_inverse(byte == 255u ? 0u : byte);
+    uint32_t q[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) q[i] = whole8(number(v[i]), inverse);
+    typedef typename Word<E>::type W;
+    W w;
+    if constexpr (E == 8) {
+        w[0] = low_bytes(q[0], q[1], q[2], q[3]);
+        w[1] = low_bytes(q[4], q[5], q[6], q[7]);
+        if (byte == 255u) w = W{0u, 0u};
+    } else {
+        w = low_bytes(q[0], q[1], q[2], q[3]);
+        if (byte == 255u) w = 0u;
+    }
+    reinterpret_cast<W*>(codes)[p.lane] = w;
+    store_scales<T>(scales, p, byte);
+    if constexpr (FN != NKMX_NONE) {
+        typename Pack<T, E>::vec o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = (T)activation<FN>(number(v[i]));
+        store_pack<T, E>(y + p.row * ldy + p.col, o, p.live);
+    }
+}
+
+template <int SEL>
+__device__ __forceinline__ void values4(uint32_t w, float scale, float& a, float& b)
+{
+    const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, SEL);
+    a = v[0];
+    b = v[1];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(T* out, uint64_t ldo, const uint8_t* codes,
+                                                             const uint8_t* scales, FastDiv steps, uint32_t n_steps,
+                                                             uint32_t cols)
+{
+    constexpr int E = Lanes<T>::E;
+    Place p;
+    if (!place_of<T>(p, steps, n_steps, cols)) return;
+    typedef typename Word<E / 2>::type W;
+    const uint32_t w = reinterpret_cast<const W*>(codes)[p.lane];
+    const uint32_t byte = scales[p.lane / Lanes<T>::block];
+    const float scale = scale_value(byte == 255u ? 127u : byte);
+    float f[8];
+    values4<0>(w, scale, f[0], f[1]);
+    values4<1>(w, scale, f[2], f[3]);
+    if constexpr (E == 8) {
+        values4<2>(w, scale, f[4], f[5]);
+        values4<3>(w, scale, f[6], f[7]);
+    }
+    typename Pack<T, E>::vec o;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = (T)(byte == 255u ? __uint_as_float(0x7FC00000u) : f[i]);
+    store_pack<T, E>(out + p.row * ldo + p.col, o, p.live);
+}
+
+// out = value of the codes (FN none) or dy * fn'(value).
+template <typename T, int FN>
+__global__ __launch_bounds__(256) void act8_grad_kernel(T* out, uint64_t ldo, const T* dy, uint64_t ldy,
+                                                        const uint8_t* codes, const uint8_t* scales, FastDiv steps,
+                                                        uint32_t n_steps, uint32_t cols)
+{
+    constexpr int E = Lanes<T>::E;
+    Place p;
+    if (!place_of<T>(p, steps, n_steps, cols)) return;
+    typename Pack<T, E>::vec g, o;
+    if constexpr (FN != NKMX_NONE) g = load_pack<T, E>(dy + p.row * ldy + p.col, p.live);
+    typedef typename Word<E>::type W;
+    const W w = reinterpret_cast<const W*>(codes)[p.lane];
+    const float scale = scale_value(scales[p.lane / Lanes<T>::block]);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        uint32_t four;
+        if constexpr (E == 8) four = w[i / 4];
+        else four = w;
+        const float v = (float)(int8_t)(four >> (8 * (i & 3))) * scale;
+        if constexpr (FN != NKMX_NONE) o[i] = (T)(number(g[i]) * activation_slope<FN>(v));
+        else o[i] = (T)v;
+    }
+    store_pack<T, E>(out + p.row * ldo + p.col, o, p.live);
+}
+
+// The transpose: blocks run down x's columns.  A workgroup of 8 waves takes 256 rows x 64 * CPL columns; a wave
+// takes 32 rows = one block of every column, a lane CPL = 2 (16-bit types, one 4-byte load a row) or 1 columns,
+// so a block never leaves its lane.  The codes cross LDS once, so that a column's 256 rows leave as 128
+// contiguous bytes: whole cache lines.
+template <typename T>
+__global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x, uint64_t ldx, uint8_t* codes,
+                                                                      uint8_t* scales, uint32_t rows, uint32_t cols,
+                                                                      uint32_t steps, uint32_t col_tiles)
+{
+    constexpr int CPL = 4 / (int)sizeof(T);
+    constexpr int TC = 64 * CPL;
+    // 16-byte slots, 8 a column: slot s of column c lies at s ^ (c & 7), so that neither side collides in the banks
+    __shared__ u32x4 image[TC * 8];
+    __shared__ alignas(16) uint8_t bytes[TC * 8];
+    const uint32_t tile = blockIdx.x % col_tiles, band = blockIdx.x / col_tiles;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint32_t r0 = band * 256 + wave * 32, c0 = tile * TC + lane * CPL;
+    const int live = (int)min((uint32_t)32, rows > r0 ? rows - r0 : 0u);
+    const int64_t live_cols = (int64_t)cols - (int64_t)c0;
+    typename Pack<T, CPL>::vec v[32];
+    const T* p = x + (uint64_t)r0 * ldx + c0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        if (i < live) {
+            v[i] = load_pack<T, CPL>(p + (uint64_t)i * ldx, live_cols);
+        } else {
+#pragma unroll
+            for (int j = 0; j < CPL; ++j) v[i][j] = (T)0.0f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = max(top, magnitude(number(v[i][j])));
+        const uint32_t byte = scale_byte<2>(top);
+        const float scale = scale_value(byte);
+        u32x4 w;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            uint32_t one = pair4<0>(0u, v[8 * d][j], v[8 * d + 1][j], scale);
+            one = pair4<1>(one, v[8 * d + 2][j], v[8 * d + 3][j], scale);
+            one = pair4<2>(one, v[8 * d + 4][j], v[8 * d + 5][j], scale);
+            one = pair4<3>(one, v[8 * d + 6][j], v[8 * d + 7][j], scale);
+            w[d] = byte == 255u ? 0u : one;
+        }
+        const int c = lane * CPL + j;
+        image[c * 8 + (wave ^ (c & 7))] = w;
+        bytes[c * 8 + wave] = (uint8_t)byte;
+    }
+    __syncthreads();
+    const uint32_t last = steps * 4;  // blocks of a packed row
+    for (int i = threadIdx.x; i < TC * 8; i += 512) {
+        const int c = i >> 3, s = i & 7;
+        if (tile * TC + c < cols && band * 8 + s < last)
+            reinterpret_cast<u32x4*>(codes)[(uint64_t)(tile * TC + c) * last + band * 8 + s] = image[c * 8 + (s ^ (c & 7))];
+    }
+    for (int i = threadIdx.x; i < TC * 2; i += 512) {  // a step's 4 scale bytes at a time
+        const int c = i >> 1, h = i & 1;
+        if (tile * TC + c < cols && band * 2 + h < steps)
+            reinterpret_cast<uint32_t*>(scales)[(uint64_t)(tile * TC + c) * steps + band * 2 + h] =
+                *reinterpret_cast<const uint32_t*>(&bytes[c * 8 + h * 4]);
+    }
+}
+
+// ---------------------------------------------------------------- mx4 product, few rows
+//
+// Few rows of a: the call reads b once and is bound by that.  A workgroup owns 16 rows of b and MT x 16 rows
+// of a; its 8 waves take the steps of k in turn, straight from memory into the operands of the matrix
+// instruction (16 x 16 x 128: lane l holds row l % 16 and block l / 16 of the step, 16 bytes as they are
+// stored), and their sums are joined through LDS in wave order.  FUSED: a lane quantizes its own block of
+// 32 numbers of x in registers, with the arithmetic of mx4_quantize_kernel.
+
+constexpr int kRowsWaves = 8;
+
+__device__ __forceinline__ i32x8 operand4(u32x4 v)
+{
+    return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+}
+
+// The block of 32 numbers that starts at p, `live` of them in the matrix, as an operand and its scale byte.
+template <typename T>
+__device__ __forceinline__ u32x4 quantize_block(const T* p, int64_t live, uint32_t& byte)
+{
+    typedef typename Pack<T, 8>::vec V;
+    typedef typename Pack<T, 8>::loose L;
+    V v[4];
+    if (live >= 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const L*>(p + 8 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i / 8][i % 8] = i < live ? p[i] : (T)0.0f;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, magnitude(number(v[i / 8][i % 8])));
+    byte = scale_byte<2>(top);
+    const float scale = scale_value(byte);
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = byte == 255u ? 0u : codes4<V, 8>(v[i], scale);
+    return w;
+}
+
+template <typename T, int MT, bool FUSED>
+__global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_t ldy, const T* x, uint64_t ldx,
+                                                                   const uint8_t* ca, const uint8_t* sa, const uint8_t* cb,
+                                                                   const uint8_t* sb, const T* bias, uint32_t m, uint32_t n,
+                                                                   uint32_t k, uint32_t steps)
+{
+    __shared__ float sums[kRowsWaves][MT][256];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+    const uint64_t row_b = min(n0 + r, n - 1);
+    const u32x4* pb = reinterpret_cast<const u32x4*>(cb) + row_b * steps * 4 + g;
+    const uint32_t* qb = reinterpret_cast<const uint32_t*>(sb) + row_b * steps;
+    f32x4 acc[MT] = {};
+    for (uint32_t s = wave; s < steps; s += kRowsWaves) {
+        const i32x8 vb = operand4(pb[s * 4]);
+        const int eb = (int)((qb[s] >> (8 * g)) & 255u);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            u32x4 a = {0u, 0u, 0u, 0u};
+            uint32_t ea = 0;
+            if constexpr (FUSED) {
+                const uint32_t row = m0 + 16 * t + r;
+                const int64_t live = (int64_t)k - (int64_t)(s * kStep + g * 32);
+                if (row < m) a = quantize_block<T>(x + row * ldx + s * kStep + g * 32, live, ea);
+            } else {
+                const uint64_t row = min(m0 + 16 * t + r, m - 1);
+                a = reinterpret_cast<const u32x4*>(ca)[(row * steps + s) * 4 + g];
+                ea = (reinterpret_cast<const uint32_t*>(sa)[row * steps + s] >> (8 * g)) & 255u;
+            }
+            acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(a), vb, acc[t], 4, 4, 0, (int)ea, 0, eb);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[wave][t][(4 * g + i) * 16 + r] = acc[t][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += 64 * kRowsWaves) {
+        float s = sums[0][i >> 8][i & 255];
+#pragma unroll
+        for (int w = 1; w < kRowsWaves; ++w) s += sums[w][i >> 8][i & 255];
+        const uint32_t row = m0 + (i >> 4), col = n0 + (i & 15);
+        if (row < m && col < n) {
+            if (bias) s += number(bias[col]);
+            y[row * ldy + col] = (T)s;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- tiles
+
+// Workgroup -> tile.  Workgroups go to the 8 XCDs in turn; each XCD takes a contiguous run of tiles, and tiles
+// run down bands of 8 tile rows, so that what is resident on one XCD shares operands in its L2.
+__device__ __forceinline__ void tile_of(uint32_t b, uint32_t row_tiles, uint32_t col_tiles, uint32_t& tr, uint32_t& tc)
+{
+    const uint32_t total = row_tiles * col_tiles, xcd = b & 7u, each = total >> 3, more = total & 7u;
+    const uint32_t t = xcd * each + min(xcd, more) + (b >> 3);
+    const uint32_t band = t / (8 * col_tiles), in = t % (8 * col_tiles);
+    const uint32_t high = min(8u, row_tiles - band * 8);
+    tr = band * 8 + in % high;
+    tc = in / high;
+}
+
+// ---------------------------------------------------------------- mx4 product, tiles
+//
+// A workgroup computes TM x TN of y in waves of WM x WN (32 x 32 x 64 matrix instructions: lane l holds row
+// l % 32 and one block of 32 columns); the steps of k go through two LDS buffers, loaded into registers one
+// step ahead.  LDS holds a tile row as 64 bytes = 4 slots of 16; slot s of row r lies at s ^ swizzle4(r), so
+// that rows a bank period apart do not meet.  The two half-steps of a lane are blocks 2g and 2g + 1 (g =
+// l / 32): any assignment of blocks to instructions is right as long as both operands agree, and in this one a
+// lane's two scale bytes are neighbours: one 16-bit LDS read, selected by the instruction's own byte index.
+
+__device__ __forceinline__ uint32_t swizzle4(uint32_t row)
+{
+    return ((row >> 1) & 2u) | (((row >> 1) ^ (row >> 3)) & 1u);
+}
+
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
+    T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb, const T* bias,
+    uint32_t m, uint32_t n, uint32_t steps, uint32_t row_tiles, uint32_t col_tiles)
+{
+    constexpr int NT = 64 * (TM / WM) * (TN / WN), WAVES_N = TN / WN;
+    constexpr int FM = WM / 32, FN = WN / 32;
+    constexpr int CHUNKS = (TM + TN) * 4 / NT;   // 16-byte pieces a thread moves per step
+    constexpr int SCALES = (TM + TN + NT - 1) / NT;
+    static_assert((TM * 4) % NT == 0 && (TN * 4) % NT == 0, "each thread's pieces belong to one operand");
+    __shared__ u32x4 image[2][(TM + TN) * 4];
+    __shared__ uint32_t bytes[2][TM + TN];
+
+    uint32_t tr, tc;
+    tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
+
+    // rows past the end read the last row: their results are not stored
+    const u32x4* from[CHUNKS];
+    const uint32_t* from_s[SCALES];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        const uint32_t c = tid + i * NT, row = c >> 2, slot = c & 3;
+        const bool is_a = row < TM;
+        const uint32_t at = is_a ? min(tr * TM + row, m - 1) : min(tc * TN + (row - TM), n - 1);
+        from[i] = reinterpret_cast<const u32x4*>(is_a ? ca : cb) + (uint64_t)at * steps * 4 + (slot ^ swizzle4(row));
+    }
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) {
+        const uint32_t row = min((uint32_t)(tid + i * NT), (uint32_t)(TM + TN - 1));
+        const bool is_a = row < TM;
+        const uint32_t at = is_a ? min(tr * TM + row, m - 1) : min(tc * TN + (row - TM), n - 1);
+        from_s[i] = reinterpret_cast<const uint32_t*>(is_a ? sa : sb) + (uint64_t)at * steps;
+    }
+    u32x4 next[CHUNKS];
+    uint32_t next_s[SCALES];
+    auto fetch = [&](uint32_t s) {
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) next[i] = from[i][(uint64_t)s * 4];
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i) next_s[i] = from_s[i][s];
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) image[buf][tid + i * NT] = next[i];
+#pragma unroll
+        for (int i = 0; i < SCALES; ++i)
+            if (tid + i * NT < TM + TN) bytes[buf][tid + i * NT] = next_s[i];
+    };
+
+    f32x16 acc[FM][FN] = {};
+    fetch(0);
+    put(0);
+    __syncthreads();
+    const uint32_t sw = swizzle4(r);  // tile rows of a fragment start at multiples of 32
+    for (uint32_t s = 0; s < steps; ++s) {
+        const int buf = s & 1;
+        if (s + 1 < steps) fetch(s + 1);
+        uint32_t ea[FM], eb[FN];
+        const uint16_t* half = reinterpret_cast<const uint16_t*>(bytes[buf]);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) ea[i] = half[(wm + 32 * i + r) * 2 + g];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) eb[j] = half[(TM + wn + 32 * j + r) * 2 + g];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            i32x8 a[FM], b[FN];
+            const uint32_t slot = (2 * g + h) ^ sw;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) a[i] = operand4(image[buf][(wm + 32 * i + r) * 4 + slot]);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) b[j] = operand4(image[buf][(TM + wn + 32 * j + r) * 4 + slot]);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    if (h == 0)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 0,
+                                                                                   (int)ea[i], 0, (int)eb[j]);
+                    else
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 1,
+                                                                                   (int)ea[i], 1, (int)eb[j]);
+                }
+        }
+        if (s + 1 < steps) put(buf ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const uint32_t col = tc * TN + wn + 32 * j + r;
+        const float add = bias && col < n ? number(bias[col]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t row = tr * TM + wm + 32 * i + 8 * (e / 4) + 4 * g + e % 4;
+                if (row < m && col < n) {
+                    float v = acc[i][j][e];
+                    if (bias) v += add;
+                    y[row * ldy + col] = (T)v;
+                }
+            }
+    }
+}
+
+// ---------------------------------------------------------------- weight gradient
+//
+// dw = dy^T x^: both operands have the contracted index (the token) as their row, so a tile has to be turned
+// before the matrix instruction can read it.  A thread loads 8 tokens x 4 columns; packing two tokens of a
+// column into one register is also the conversion to bf16 pairs, so the turn is free; a column's 8 tokens go
+// to LDS as one 16-byte slot.  x^ = q 2^e has at most 7 bits and is exact in bf16.  dy is cut into PARTS
+// bf16 numbers by truncation (1 for bf16, 2 for fp16, 3 for fp32: 8 bits each, exact together), each
+// multiplied with x^ in turn: exact products for every type at the bf16 rate, where the fp32 matrix
+// instruction has a sixteenth of it.
+//
+// LDS: column c of a tile is BT tokens = BT / 8 slots; slot s lies at s ^ swizzle_t(c).  t is split over
+// blockIdx.y where there are few tiles; the parts are joined in order by a second kernel.
+
+template <int SLOTS>
+__device__ __forceinline__ uint32_t swizzle_t(uint32_t c)
+{
+    if constexpr (SLOTS == 8) return ((c >> 2) ^ c) & 7u;
+    return ((c >> 1) & 2u) | (((c >> 1) ^ (c >> 3)) & 1u);
+}
+
+// Two tokens' upper halves side by side (the lower half of the register is the first token).
+__device__ __forceinline__ uint32_t upper_halves(uint32_t first, uint32_t second)
+{
+    return __builtin_amdgcn_perm(second, first, 0x07060302u);
+}
+__device__ __forceinline__ uint32_t lower_halves(uint32_t first, uint32_t second)
+{
+    return __builtin_amdgcn_perm(second, first, 0x05040100u);
+}
+
+// What is left of v after its upper 8 significant bits.  An infinity leaves nothing, a NaN a NaN.
+__device__ __forceinline__ float rest_of(float v)
+{
+    const float left = v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+    return magnitude(v) == kInfBits ? 0.0f : left;
+}
+
+template <typename T>
+struct Parts;
+template <>
+struct Parts<bf16> { static constexpr int count = 1; };
+template <>
+struct Parts<f16> { static constexpr int count = 2; };
+template <>
+struct Parts<float> { static constexpr int count = 3; };
+
+template <typename T, int TN, int TK, int WN, int WK, int BT>
+__global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
+    float* dw, uint64_t lddw, float* db, const T* dy, uint64_t lddy, const uint8_t* codes, const uint8_t* scales,
+    uint32_t t_rows, uint32_t n, uint32_t k, uint32_t steps, uint32_t row_tiles, uint32_t col_tiles,
+    uint32_t stages_each, uint32_t accumulate, uint64_t part_stride, uint64_t part_stride_db)
+{
+    constexpr int NT = 64 * (TN / WN) * (TK / WK), WAVES_K = TK / WK, P = Parts<T>::count;
+    constexpr int FN = WN / 32, FK = WK / 32, SLOTS = BT / 8;
+    constexpr int UD = SLOTS * (TN / 4), UX = SLOTS * (TK / 4);  // units of 8 tokens x 4 columns
+    constexpr bool BOTH = UD >= NT;                              // a thread has a unit of each, or one of one
+    static_assert(BOTH ? (UD == NT && UX == NT) : (UD + UX <= NT && UD % 64 == 0), "units and threads");
+    __shared__ u32x4 left[2][P][TN * SLOTS];
+    __shared__ u32x4 right[2][TK * SLOTS];
+
+    uint32_t tr, tc;
+    tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wn = (wave / WAVES_K) * WN, wk = (wave % WAVES_K) * WK;
+    const uint32_t stages = (t_rows + BT - 1) / BT;
+    const uint32_t first = blockIdx.y * stages_each, last = min(stages, first + stages_each);
+
+    const bool has_d = BOTH || tid < UD, has_x = BOTH || (tid >= UD && tid < UD + UX);
+    const int ud = tid, ux = BOTH ? tid : tid - UD;
+    const int d_slot = ud / (TN / 4), d_col = (ud % (TN / 4)) * 4;
+    const int x_slot = ux / (TK / 4), x_col = (ux % (TK / 4)) * 4;
+    const int64_t live_d = (int64_t)n - (int64_t)(tr * TN + d_col);
+    const uint32_t col_x = tc * TK + x_col;
+    const bool live_x = has_x && col_x < steps * kStep;
+    const bool sums_dy = db != nullptr && tc == 0 && has_d;
+
+    typename Pack<T, 4>::vec d[8];
+    uint32_t q[8];
+    uint8_t e[8];
+    auto fetch = [&](uint32_t stage) {
+        if (has_d) {
+            const uint32_t t0 = stage * BT + d_slot * 8;
+            const T* p = dy + (uint64_t)t0 * lddy + tr * TN + d_col;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                d[i] = typename Pack<T, 4>::vec{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+                if (t0 + i < t_rows && live_d > 0) {
+                    if (live_d >= 4) {
+                        d[i] = *reinterpret_cast<const typename Pack<T, 4>::loose*>(p + (uint64_t)i * lddy);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 3; ++j)
+                            if (j < live_d) d[i][j] = p[(uint64_t)i * lddy + j];
+                    }
+                }
+            }
+        }
+        if (has_x) {
+            const uint32_t t0 = stage * BT + x_slot * 8;
+            const uint8_t* p = codes + (uint64_t)t0 * steps * kStep + col_x;
+            const uint8_t* ps = scales + (uint64_t)t0 * steps * 4 + col_x / 32;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[i] = 0u;
+                e[i] = 0;
+                if (live_x && t0 + i < t_rows) {
+                    q[i] = *reinterpret_cast<const uint32_t*>(p + (uint64_t)i * steps * kStep);
+                    e[i] = ps[(uint64_t)i * steps * 4];
+                }
+            }
+        }
+    };
+    float sum_dy[4] = {};
+    auto put = [&](int buf) {
+        if (has_d) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t c = d_col + j, at = c * SLOTS + (d_slot ^ swizzle_t<SLOTS>(c));
+                if (sums_dy) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum_dy[j] += number(d[i][j]);
+                }
+                if constexpr (P == 1) {
+                    u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a = __builtin_bit_cast(u32x2, d[2 * i])[j / 2];
+                        const uint32_t b = __builtin_bit_cast(u32x2, d[2 * i + 1])[j / 2];
+                        w[i] = j % 2 ? upper_halves(a, b) : lower_halves(a, b);
+                    }
+                    left[buf][0][at] = w;
+                } else {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = number(d[i][j]);
+#pragma unroll
+                    for (int part = 0; part < P; ++part) {
+                        u32x4 w;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = upper_halves(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
+                        left[buf][part][at] = w;
+                        if (part + 1 < P) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[i] = rest_of(v[i]);
+                        }
+                    }
+                }
+            }
+        }
+        if (has_x) {
+            float s[8], zero[8];
+            uint32_t u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s[i] = scale_value(e[i]);
+                zero[i] = -128.0f * s[i];
+                u[i] = q[i] ^ 0x80808080u;  // q + 128 as an unsigned byte: one conversion each
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t c = x_col + j;
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = fmaf((float)((u[2 * i] >> (8 * j)) & 255u), s[2 * i], zero[2 * i]);
+                    const float b = fmaf((float)((u[2 * i + 1] >> (8 * j)) & 255u), s[2 * i + 1], zero[2 * i + 1]);
+                    w[i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)a, (bf16)b});
+                }
+                right[buf][c * SLOTS + (x_slot ^ swizzle_t<SLOTS>(c))] = w;
+            }
+        }
+    };
+
+    f32x16 acc[FN][FK] = {};
+    if (first < last) {
+        fetch(first);
+        put(0);
+    }
+    __syncthreads();
+    for (uint32_t s = first; s < last; ++s) {
+        const int buf = (s - first) & 1;
+        if (s + 1 < last) fetch(s + 1);
+#pragma unroll
+        for (int h = 0; h < BT / 16; ++h) {
+            bf16x8 b[FK];
+#pragma unroll
+            for (int j = 0; j < FK; ++j) {
+                const uint32_t c = wk + 32 * j + r;
+                b[j] = __builtin_bit_cast(bf16x8, right[buf][c * SLOTS + ((2 * h + g) ^ swizzle_t<SLOTS>(c))]);
+            }
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const uint32_t c = wn + 32 * i + r;
+#pragma unroll
+                for (int part = P - 1; part >= 0; --part) {  // smallest first
+                    const bf16x8 a =
+                        __builtin_bit_cast(bf16x8, left[buf][part][c * SLOTS + ((2 * h + g) ^ swizzle_t<SLOTS>(c))]);
+#pragma unroll
+                    for (int j = 0; j < FK; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+        if (s + 1 < last) put(buf ^ 1);
+        __syncthreads();
+    }
+
+    float* out = dw + blockIdx.y * part_stride;
+#pragma unroll
+    for (int j = 0; j < FK; ++j) {
+        const uint32_t col = tc * TK + wk + 32 * j + r;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const uint32_t row = tr * TN + wn + 32 * i + 8 * (v / 4) + 4 * g + v % 4;
+                if (row < n && col < k) {
+                    float* p = out + row * lddw + col;
+                    *p = accumulate ? *p + acc[i][j][v] : acc[i][j][v];
+                }
+            }
+    }
+    if (db != nullptr && tc == 0) {  // the token groups' sums of a column, joined in order
+        float* part = reinterpret_cast<float*>(&right[0][0]);
+        if (has_d) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) part[d_slot * TN + d_col + j] = sum_dy[j];
+        }
+        __syncthreads();
+        if (tid < TN && tr * TN + tid < n) {
+            float s = part[tid];
+#pragma unroll
+            for (int i = 1; i < SLOTS; ++i) s += part[i * TN + tid];
+            float* p = db + blockIdx.y * part_stride_db + tr * TN + tid;
+            *p = accumulate ? *p + s : s;
+        }
+    }
+}
+
+// Joins the parts of a split weight gradient, [parts][rows][cols] in the workspace, in order.
+__global__ __launch_bounds__(256) void join_parts_kernel(float* out, uint64_t ldo, const float* part, uint32_t parts,
+                                                         uint64_t part_stride, uint32_t rows, uint32_t cols,
+                                                         uint64_t ldp, uint32_t accumulate)
+{
+    const uint32_t per_row = (cols + 3) / 4;
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t row = i / per_row;
+    if (row >= rows) return;
+    const uint32_t col = (uint32_t)(i % per_row) * 4;
+    const int64_t live = (int64_t)cols - (int64_t)col;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t p = 0; p < parts; ++p) {  // rows of the workspace are padded to whole quads
+        const f32x4 v = *reinterpret_cast<const f32x4*>(part + p * part_stride + row * ldp + col);
+        s = p ? s + v : v;
+    }
+    float* o = out + row * ldo + col;
+    if (accumulate) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < live) s[j] = o[j] + s[j];
+    }
+    store_pack<float, 4>(o, s, live);
+}
+
+// ---------------------------------------------------------------- host side
+
+// hipLaunchKernel returns what THIS launch did; the runtime's "last error" is left alone unless the launch
+// failed (then it is cleared, since the failure is reported through the return value).
+template <typename Tuple, size_t... I>
+inline void arg_pointers(Tuple& vals, void** out, std::index_sequence<I...>)
+{
+    ((out[I] = static_cast<void*>(&std::get<I>(vals))), ...);
+}
+
+template <typename... KArgs, typename... Args>
+inline int launch(void (*kernel)(KArgs...), dim3 grid, uint32_t block, hipStream_t s, Args... args)
+{
+    static_assert(sizeof...(KArgs) == sizeof...(Args), "kernel argument count");
+    std::tuple<KArgs...> vals(static_cast<KArgs>(args)...);
+    void* ptrs[sizeof...(KArgs)];
+    arg_pointers(vals, ptrs, std::index_sequence_for<KArgs...>{});
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(block), ptrs, 0, s);
+    if (e != hipSuccess) (void)hipGetLastError();
+    return e == hipSuccess ? NKMX_OK : (int)e;
+}
+
+constexpr uint64_t kMaxSize = 0x7FFFFFFFull;
+inline uint64_t steps_of(uint64_t cols) { return (cols + kStep - 1) / kStep; }
+inline uint64_t size_of(int type) { return type == NKMX_F32 ? 4 : 2; }
+inline bool known_type(int type) { return type == NKMX_F32 || type == NKMX_BF16 || type == NKMX_F16; }
+inline bool on(const void* p, uint64_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) == 0; }
+
+// A buffer of a call: rows of `width` bytes, `pitch` apart.
+struct Area {
+    uintptr_t at;
+    uint64_t rows, width, pitch;
+};
+inline Area area(const void* p, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t size)
+{
+    return Area{reinterpret_cast<uintptr_t>(p), rows, cols * size, ld * size};
+}
+inline Area run(const void* p, uint64_t bytes) { return Area{reinterpret_cast<uintptr_t>(p), 1, bytes, bytes}; }
+
+// Whether two buffers share a byte.  Two matrices with the same leading dimension may interleave (column
+// ranges of one larger matrix); otherwise the whole extents count.
+inline bool overlap(const Area& a, const Area& b)
+{
+    if (!a.rows || !b.rows || !a.width || !b.width) return false;
+    const uintptr_t ea = a.at + (a.rows - 1) * a.pitch + a.width, eb = b.at + (b.rows - 1) * b.pitch + b.width;
+    if (ea <= b.at || eb <= a.at) return false;
+    if (a.rows > 1 && b.rows > 1 && a.pitch == b.pitch) {
+        const uint64_t off = b.at >= a.at ? (b.at - a.at) % a.pitch : (a.pitch - (a.at - b.at) % a.pitch) % a.pitch;
+        return !(off >= a.width && off + b.width <= a.pitch);
+    }
+    return true;
+}
+inline bool same(const Area& a, const Area& b)
+{
+    return a.at == b.at && a.rows == b.rows && a.width == b.width && (a.rows <= 1 || a.pitch == b.pitch);
+}
+
+// Calls f with a null pointer of the element type.
+template <typename F>
+inline int for_type(int type, F f)
+{
+    switch (type) {
+        case NKMX_F32: return f((float*)nullptr);
+        case NKMX_BF16: return f((bf16*)nullptr);
+        default: return f((f16*)nullptr);
+    }
+}
+
+// The streaming launches: steps of the packed matrix, lanes, workgroups.
+struct Stream {
+    FastDiv steps;
+    uint32_t n_steps, cols, blocks;
+};
+template <typename T>
+inline bool stream_of(Stream& s, uint64_t rows, uint64_t cols)
+{
+    const uint64_t steps = steps_of(cols), total = rows * steps;  // both below 2^31
+    if (total > 0xFFFFFFFFull) return false;
+    const uint64_t blocks = (total * Lanes<T>::step + 255) / 256;
+    if (blocks > kMaxSize) return false;
+    s = Stream{fast_div((uint32_t)steps), (uint32_t)total, (uint32_t)cols, (uint32_t)blocks};
+    return true;
+}
+
+// The rules on matrices of numbers: sizes, leading dimension, alignment.
+inline int check_matrix(const void* p, int type, uint64_t rows, uint64_t cols, uint64_t ld)
+{
+    if (rows > kMaxSize || cols > kMaxSize || ld > kMaxSize || (rows > 1 && ld < cols)) return NKMX_ERANGE;
+    if (rows == 0 || cols == 0) return NKMX_OK;
+    if (!p) return NKMX_ENULL;
+    return on(p, size_of(type)) ? NKMX_OK : NKMX_EALIGN;
+}
+inline int check_packed(const void* codes, const void* scales, uint64_t rows, uint64_t cols)
+{
+    if (rows > kMaxSize || cols > kMaxSize) return NKMX_ERANGE;
+    if (rows == 0 || cols == 0) return NKMX_OK;
+    if (!codes || !scales) return NKMX_ENULL;
+    return on(codes, 16) && on(scales, 4) ? NKMX_OK : NKMX_EALIGN;
+}
+inline Area codes4(const void* p, uint64_t rows, uint64_t cols) { return run(p, rows * steps_of(cols) * kStepBytes4); }
+inline Area codes8(const void* p, uint64_t rows, uint64_t cols) { return run(p, rows * steps_of(cols) * kStep); }
+inline Area scale_bytes(const void* p, uint64_t rows, uint64_t cols) { return run(p, rows * steps_of(cols) * 4); }
+
+#define NKMX_TRY(call)                 \
+    do {                               \
+        const int rc_ = (call);        \
+        if (rc_ != NKMX_OK) return rc_; \
+    } while (0)
+
+// ---- product
+
+constexpr uint64_t kRowsMax = 64;       // rows of a that the few-rows kernel takes
+constexpr uint64_t kFusedRowsMax = 8;   // rows of x that are quantized inside the product
+
+template <typename T, int MT, bool FUSED>
+inline int launch_rows(T* y, uint64_t ldy, const T* x, uint64_t ldx, const uint8_t* ca, const uint8_t* sa,
+                       const uint8_t* cb, const uint8_t* sb, const T* bias, uint64_t m, uint64_t n, uint64_t k,
+                       hipStream_t s)
+{
+    const dim3 grid((uint32_t)((n + 15) / 16), (uint32_t)((m + 16 * MT - 1) / (16 * MT)));
+    return launch(mx4_rows_kernel<T, MT, FUSED>, grid, 64 * kRowsWaves, s, y, ldy, x, ldx, ca, sa, cb, sb, bias,
+                  (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)steps_of(k));
+}
+
+template <typename T, int TM, int TN, int WM, int WN>
+inline int launch_tiles(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb,
+                        const T* bias, uint64_t m, uint64_t n, uint64_t k, hipStream_t s)
+{
+    const uint64_t rt = (m + TM - 1) / TM, ct = (n + TN - 1) / TN;
+    if (rt * ct > kMaxSize) return NKMX_ERANGE;
+    return launch(mx4_tiles_kernel<T, TM, TN, WM, WN>, dim3((uint32_t)(rt * ct)), 64 * (TM / WM) * (TN / WN), s, y, ldy,
+                  ca, sa, cb, sb, bias, (uint32_t)m, (uint32_t)n, (uint32_t)steps_of(k), (uint32_t)rt, (uint32_t)ct);
+}
+
+template <typename T>
+int product(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb,
+            const T* bias, uint64_t m, uint64_t n, uint64_t k, hipStream_t s)
+{
+    if (k == 0 || m <= kRowsMax) {
+        if (m <= 16) return launch_rows<T, 1, false>(y, ldy, nullptr, 0, ca, sa, cb, sb, bias, m, n, k, s);
+        if (m <= 32) return launch_rows<T, 2, false>(y, ldy, nullptr, 0, ca, sa, cb, sb, bias, m, n, k, s);
+        return launch_rows<T, 4, false>(y, ldy, nullptr, 0, ca, sa, cb, sb, bias, m, n, k, s);
+    }
+    const auto tiles = [&](uint64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
+    if (tiles(256) >= 192) return launch_tiles<T, 256, 256, 128, 64>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    if (tiles(128) >= 192) return launch_tiles<T, 128, 128, 64, 64>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    return launch_tiles<T, 64, 64, 32, 32>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+}
+
+// ---- weight gradient
+
+struct WgradPlan {
+    int side;              // tile: 256, 128 or 64
+    uint64_t row_tiles, col_tiles, parts, stages_each, ldp;
+    uint64_t part_floats;  // of dw and db of one part in the workspace
+};
+
+WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
+{
+    const auto tiles = [&](uint64_t side) { return ((n + side - 1) / side) * ((k + side - 1) / side); };
+    WgradPlan p = {};
+    p.side = tiles(256) * ((t + 1023) / 1024) >= 256 ? 256 : (tiles(128) * ((t + 511) / 512) >= 128 ? 128 : 64);
+    const uint64_t bt = p.side == 256 && type != NKMX_BF16 ? 32 : 64;
+    const uint64_t stages = (t + bt - 1) / bt, count = tiles(p.side);
+    p.row_tiles = (n + p.side - 1) / p.side;
+    p.col_tiles = (k + p.side - 1) / p.side;
+    // split t until the tiles fill the chip, but keep 8 stages a part
+    uint64_t parts = count ? 256 / count : 1;
+    if (parts > stages / 8) parts = stages / 8;
+    if (parts < 1) parts = 1;
+    p.stages_each = (stages + parts - 1) / parts;
+    p.parts = p.stages_each ? (stages + p.stages_each - 1) / p.stages_each : 1;
+    if (p.parts < 1) p.parts = 1;
+    p.ldp = (k + 3) / 4 * 4;
+    p.part_floats = n * p.ldp + (n + 3) / 4 * 4;
+    return p;
+}
+
+template <typename T, int TN, int TK, int WN, int WK, int BT>
+inline int launch_wgrad(const WgradPlan& p, float* dw, uint64_t lddw, float* db, const T* dy, uint64_t lddy,
+                        const uint8_t* codes, const uint8_t* scales, uint64_t t, uint64_t n, uint64_t k,
+                        uint32_t accumulate, uint64_t stride, hipStream_t s)
+{
+    const uint64_t tiles = p.row_tiles * p.col_tiles;
+    if (tiles > kMaxSize || p.parts > 65535) return NKMX_ERANGE;
+    return launch(act8_wgrad_kernel<T, TN, TK, WN, WK, BT>, dim3((uint32_t)tiles, (uint32_t)p.parts),
+                  64 * (TN / WN) * (TK / WK), s, dw, lddw, db, dy, lddy, codes, scales, (uint32_t)t, (uint32_t)n,
+                  (uint32_t)k, (uint32_t)steps_of(k), (uint32_t)p.row_tiles, (uint32_t)p.col_tiles,
+                  (uint32_t)p.stages_each, accumulate, stride, stride);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nkmx_version(void) { return NKMX_VERSION; }
+
+const char* nkmx_strerror(int code)
+{
+    switch (code) {
+        case NKMX_OK: return "success";
+        case NKMX_ENULL: return "nkmx: a required pointer is NULL";
+        case NKMX_EALIGN: return "nkmx: a pointer is not aligned (codes 16 bytes, scales 4, numbers their size)";
+        case NKMX_ERANGE: return "nkmx: a size, leading dimension, type or activation is out of range";
+        case NKMX_EALIAS: return "nkmx: an output overlaps another buffer of the call";
+        case NKMX_EWORK: return "nkmx: the workspace is missing, too small or not on a 16-byte boundary";
+        default: break;
+    }
+    if (code > 0) return hipGetErrorString((hipError_t)code);
+    return "nkmx: unknown error";
+}
+
+int nkmx_mx4_quantize(const void* x, int type, uint64_t rows, uint64_t cols, uint64_t ldx, uint8_t* codes,
+                      uint8_t* scales, int transpose, void* stream)
+{
+    if (!known_type(type)) return NKMX_ERANGE;
+    NKMX_TRY(check_matrix(x, type, rows, cols, ldx));
+    if (rows == 0 || cols == 0) return NKMX_OK;
+    const uint64_t pr = transpose ? cols : rows, pc = transpose ? rows : cols;  // of the packed matrix
+    NKMX_TRY(check_packed(codes, scales, pr, pc));
+    const Area ax = area(x, rows, cols, ldx, size_of(type)), ac = codes4(codes, pr, pc), as = scale_bytes(scales, pr, pc);
+    if (overlap(ax, ac) || overlap(ax, as) || overlap(ac, as)) return NKMX_EALIAS;
+    const hipStream_t s = (hipStream_t)stream;
+    return for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        if (transpose) {
+            constexpr uint64_t tc = 64 * (4 / sizeof(T));
+            const uint64_t tiles = (cols + tc - 1) / tc, bands = (rows + 255) / 256;
+            if (tiles * bands > kMaxSize) return NKMX_ERANGE;
+            return launch(mx4_quantize_transposed_kernel<T>, dim3((uint32_t)(tiles * bands)), 512, s, (const T*)x, ldx,
+                          codes, scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)steps_of(rows), (uint32_t)tiles);
+        }
+        Stream g;
+        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
+        return launch(mx4_quantize_kernel<T>, dim3(g.blocks), 256, s, (const T*)x, ldx, codes, scales, g.steps, g.n_steps,
+                      g.cols);
+    });
+}
+
+int nkmx_mx4_dequantize(void* out, int type, uint64_t rows, uint64_t cols, uint64_t ldo, const uint8_t* codes,
+                        const uint8_t* scales, void* stream)
+{
+    if (!known_type(type)) return NKMX_ERANGE;
+    NKMX_TRY(check_matrix(out, type, rows, cols, ldo));
+    NKMX_TRY(check_packed(codes, scales, rows, cols));
+    if (rows == 0 || cols == 0) return NKMX_OK;
+    const Area ao = area(out, rows, cols, ldo, size_of(type));
+    if (overlap(ao, codes4(codes, rows, cols)) || overlap(ao, scale_bytes(scales, rows, cols))) return NKMX_EALIAS;
+    return for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        Stream g;
+        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
+        return launch(mx4_dequantize_kernel<T>, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, codes, scales,
+                      g.steps, g.n_steps, g.cols);
+    });
+}
+
+int nkmx_mx4_matmul(void* y, int type, uint64_t m, uint64_t n, uint64_t k, uint64_t ldy, const uint8_t* a_codes,
+                    const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales, const void* bias,
+                    void* stream)
+{
+    if (!known_type(type)) return NKMX_ERANGE;
+    NKMX_TRY(check_matrix(y, type, m, n, ldy));
+    if (m == 0 || n == 0) return NKMX_OK;
+    NKMX_TRY(check_packed(a_codes, a_scales, m, k));
+    NKMX_TRY(check_packed(b_codes, b_scales, n, k));
+    if (bias && !on(bias, size_of(type))) return NKMX_EALIGN;
+    const Area ay = area(y, m, n, ldy, size_of(type));
+    if (overlap(ay, codes4(a_codes, m, k)) || overlap(ay, scale_bytes(a_scales, m, k)) ||
+        overlap(ay, codes4(b_codes, n, k)) || overlap(ay, scale_bytes(b_scales, n, k)) ||
+        (bias && overlap(ay, run(bias, n * size_of(type)))))
+        return NKMX_EALIAS;
+    return for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        return product<T>((T*)y, ldy, a_codes, a_scales, b_codes, b_scales, (const T*)bias, m, n, k, (hipStream_t)stream);
+    });
+}
+
+uint64_t nkmx_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k)
+{
+    if (m <= kFusedRowsMax || m > kMaxSize || n == 0 || n > kMaxSize || k > kMaxSize) return 0;
+    return m * steps_of(k) * (kStepBytes4 + 4);
+}
+
+int nkmx_mx4_linear(void* y, const void* x, int type, uint64_t m, uint64_t n, uint64_t k, uint64_t ldy, uint64_t ldx,
+                    const uint8_t* b_codes, const uint8_t* b_scales, const void* bias, void* workspace,
+                    uint64_t workspace_bytes, void* stream)
+{
+    if (!known_type(type)) return NKMX_ERANGE;
+    NKMX_TRY(check_matrix(y, type, m, n, ldy));
+    NKMX_TRY(check_matrix(x, type, m, k, ldx));
+    if (m == 0 || n == 0) return NKMX_OK;
+    NKMX_TRY(check_packed(b_codes, b_scales, n, k));
+    if (bias && !on(bias, size_of(type))) return NKMX_EALIGN;
+    const uint64_t need = nkmx_mx4_linear_workspace(m, n, k);
+    if (need && (!workspace || workspace_bytes < need || !on(workspace, 16))) return NKMX_EWORK;
+    const Area ay = area(y, m, n, ldy, size_of(type)), ax = area(x, m, k, ldx, size_of(type)), aw = run(workspace, need);
+    const Area ac = codes4(b_codes, n, k), as = scale_bytes(b_scales, n, k), ab = run(bias, bias ? n * size_of(type) : 0);
+    if (overlap(ay, ax) || overlap(ay, ac) || overlap(ay, as) || overlap(ay, ab) || overlap(aw, ay) || overlap(aw, ax) ||
+        overlap(aw, ac) || overlap(aw, as) || overlap(aw, ab))
+        return NKMX_EALIAS;
+    const hipStream_t s = (hipStream_t)stream;
+    uint8_t* ca = (uint8_t*)workspace;
+    uint8_t* sa = ca + m * steps_of(k) * kStepBytes4;
+    if (need) NKMX_TRY(nkmx_mx4_quantize(x, type, m, k, ldx, ca, sa, 0, stream));
+    return for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        if (m <= kFusedRowsMax && k)
+            return launch_rows<T, 1, true>((T*)y, ldy, (const T*)x, ldx, nullptr, nullptr, b_codes, b_scales,
+                                           (const T*)bias, m, n, k, s);
+        return product<T>((T*)y, ldy, ca, sa, b_codes, b_scales, (const T*)bias, m, n, k, s);
+    });
+}
+
+int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint64_t cols, uint64_t ldx, uint64_t ldy,
+                   uint8_t* codes, uint8_t* scales, void* stream)
+{
+    if (!known_type(type) || fn < NKMX_NONE || fn > NKMX_SILU) return NKMX_ERANGE;
+    NKMX_TRY(check_matrix(x, type, rows, cols, ldx));
+    if (fn != NKMX_NONE) NKMX_TRY(check_matrix(y, type, rows, cols, ldy));
+    NKMX_TRY(check_packed(codes, scales, rows, cols));
+    if (rows == 0 || cols == 0) return NKMX_OK;
+    const uint64_t b = size_of(type);
+    const Area ax = area(x, rows, cols, ldx, b), ay = area(y, fn == NKMX_NONE ? 0 : rows, cols, ldy, b);
+    const Area ac = codes8(codes, rows, cols), as = scale_bytes(scales, rows, cols);
+    if (overlap(ac, ax) || overlap(as, ax) || overlap(ac, as) || overlap(ac, ay) || overlap(as, ay) ||
+        (overlap(ay, ax) && !same(ay, ax)))
+        return NKMX_EALIAS;
+    return for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        Stream g;
+        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
+        const auto with = [&](auto kernel) {
+            return launch(kernel, dim3(g.blocks), 256, (hipStream_t)stream, (const T*)x, ldx, (T*)y, ldy, codes, scales,
+                          g.steps, g.n_steps, g.cols);
+        };
+        if (fn == NKMX_GELU) return with(act8_save_kernel<T, NKMX_GELU>);
+        if (fn == NKMX_SILU) return with(act8_save_kernel<T, NKMX_SILU>);
+        return with(act8_save_kernel<T, NKMX_NONE>);
+    });
+}
+
+static int act8_read(void* out, const void* dy, int type, int fn, uint64_t rows, uint64_t cols, uint64_t ldo,
+                     uint64_t lddy, const uint8_t* codes, const uint8_t* scales, void* stream)
+{
+    NKMX_TRY(check_matrix(out, type, rows, cols, ldo));
+    if (fn != NKMX_NONE) NKMX_TRY(check_matrix(dy, type, rows, cols, lddy));
+    NKMX_TRY(check_packed(codes, scales, rows, cols));
+    if (rows == 0 || cols == 0) return NKMX_OK;
+    const uint64_t b = size_of(type);
+    const Area ao = area(out, rows, cols, ldo, b), ad = area(dy, fn == NKMX_NONE ? 0 : rows, cols, lddy, b);
+    if (overlap(ao, codes8(codes, rows, cols)) || overlap(ao, scale_bytes(scales, rows, cols)) ||
+        (overlap(ao, ad) && !same(ao, ad)))
+        return NKMX_EALIAS;
+    return for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        Stream g;
+        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
+        const auto with = [&](auto kernel) {
+            return launch(kernel, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, (const T*)dy, lddy, codes,
+                          scales, g.steps, g.n_steps, g.cols);
+        };
+        if (fn == NKMX_GELU) return with(act8_grad_kernel<T, NKMX_GELU>);
+        if (fn == NKMX_SILU) return with(act8_grad_kernel<T, NKMX_SILU>);
+        return with(act8_grad_kernel<T, NKMX_NONE>);
+    });
+}
+
+int nkmx_act8_load(void* out, int type, uint64_t rows, uint64_t cols, uint64_t ldo, const uint8_t* codes,
+                   const uint8_t* scales, void* stream)
+{
+    if (!known_type(type)) return NKMX_ERANGE;
+    return act8_read(out, nullptr, type, NKMX_NONE, rows, cols, ldo, 0, codes, scales, stream);
+}
+
+int nkmx_act8_grad(void* dx, const void* dy, int type, int fn, uint64_t rows, uint64_t cols, uint64_t lddx,
+                   uint64_t lddy, const uint8_t* codes, const uint8_t* scales, void* stream)
+{
+    if (!known_type(type) || (fn != NKMX_GELU && fn != NKMX_SILU)) return NKMX_ERANGE;
+    return act8_read(dx, dy, type, fn, rows, cols, lddx, lddy, codes, scales, stream);
+}
+
+uint64_t nkmx_act8_wgrad_workspace(int type, uint64_t t, uint64_t n, uint64_t k)
+{
+    if (!known_type(type) || t > kMaxSize || n > kMaxSize || k > kMaxSize || n == 0) return 0;
+    const WgradPlan p = wgrad_plan(type, t, n, k);
+    return p.parts > 1 ? p.parts * p.part_floats * 4 : 0;
+}
+
+int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, uint64_t n, uint64_t k, uint64_t lddw,
+                    uint64_t lddy, const uint8_t* codes, const uint8_t* scales, int accumulate, void* workspace,
+                    uint64_t workspace_bytes, void* stream)
+{
+    if (!known_type(type)) return NKMX_ERANGE;
+    NKMX_TRY(check_matrix(dw, NKMX_F32, n, k, lddw));
+    NKMX_TRY(check_matrix(dy, type, t, n, lddy));
+    NKMX_TRY(check_packed(codes, scales, t, k));
+    if (db && !on(db, 4)) return NKMX_EALIGN;
+    if (n == 0 || (k == 0 && !db)) return NKMX_OK;
+    const uint64_t need = nkmx_act8_wgrad_workspace(type, t, n, k);
+    if (need && (!workspace || workspace_bytes < need || !on(workspace, 16))) return NKMX_EWORK;
+    const Area aw = area(dw, n, k, lddw, 4), ab = run(db, db ? n * 4 : 0), ad = area(dy, t, n, lddy, size_of(type));
+    const Area ac = codes8(codes, t, k), as = scale_bytes(scales, t, k), ak = run(workspace, need);
+    for (const Area* o : {&aw, &ab, &ak})
+        if (overlap(*o, ad) || overlap(*o, ac) || overlap(*o, as)) return NKMX_EALIAS;
+    if (overlap(aw, ab) || overlap(aw, ak) || overlap(ab, ak)) return NKMX_EALIAS;
+    const hipStream_t s = (hipStream_t)stream;
+    WgradPlan p = wgrad_plan(type, t, n, k);
+    if (p.col_tiles == 0) p.col_tiles = 1;  // k = 0: db alone
+    const bool split = p.parts > 1;
+    float* part = (float*)workspace;
+    float* to = split ? part : dw;
+    float* to_db = !db ? nullptr : (split ? part + n * p.ldp : db);
+    const uint64_t ld = split ? p.ldp : lddw, stride = split ? p.part_floats : 0;
+    const uint32_t add = !split && accumulate ? 1u : 0u;
+    NKMX_TRY(for_type(type, [&](auto* null) -> int {
+        typedef std::remove_pointer_t<decltype(null)> T;
+        constexpr int BT = Parts<T>::count == 1 ? 64 : 32;
+        if (p.side == 256)
+            return launch_wgrad<T, 256, 256, 128, 64, BT>(p, to, ld, to_db, (const T*)dy, lddy, codes, scales, t, n, k, add,
+                                                          stride, s);
+        if (p.side == 128)
+            return launch_wgrad<T, 128, 128, 64, 64, 64>(p, to, ld, to_db, (const T*)dy, lddy, codes, scales, t, n, k, add,
+                                                         stride, s);
+        return launch_wgrad<T, 64, 64, 32, 32, 64>(p, to, ld, to_db, (const T*)dy, lddy, codes, scales, t, n, k, add,
+                                                   stride, s);
+    }));
+    if (!split) return NKMX_OK;
+    const auto join = [&](float* out, uint64_t ldo, const float* from, uint64_t rows, uint64_t cols, uint64_t ldp) -> int {
+        const uint64_t blocks = (rows * ((cols + 3) / 4) + 255) / 256;
+        if (blocks > kMaxSize) return NKMX_ERANGE;
+        return launch(join_parts_kernel, dim3((uint32_t)blocks), 256, s, out, ldo, from, (uint32_t)p.parts, p.part_floats,
+                      (uint32_t)rows, (uint32_t)cols, ldp, accumulate ? 1u : 0u);
+    };
+    if (k) NKMX_TRY(join(dw, lddw, part, n, k, p.ldp));
+    if (db) NKMX_TRY(join(db, n, part + n * p.ldp, 1, n, n));
+    return NKMX_OK;
+}
+
+}  // extern "C"

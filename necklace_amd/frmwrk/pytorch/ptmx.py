@@ -1,0 +1,164 @@
+"""Layers whose stored tensors are microscaled: what a training step keeps between forward and backward, and what a
+product reads, in 8 and 4 bits.  Beside ptcomp (which packs the gradients a step sends), on the kernels of
+necklace_amd.cuda.mx.
+
+    act8_linear(x, weight, bias)   y = x W^T + b by torch; x is kept in 8 bits and the weight gradient read from it
+    act8_act(x, fn)                y = fn(x), "gelu" or "silu"; x is kept in 8 bits and the gradient read from it
+    mx4_linear(x, weight, bias)    y = mx4(x) mx4(W)^T + b; backward dx = mx4(dy) mx4(W^T)^T, dW as in act8_linear:
+                                   the rounding is treated as the identity (straight through)
+    Mx4Weight(weight)              the codes alone, laid out once: .linear(x, bias) for serving
+
+x is float32, bfloat16 or float16 on the GPU, [..., in]; weight [out, in] and bias [out] of the same type.  Gradients
+have their tensor's type; the weight gradient is summed in fp32 whatever that is.  The calls run on torch's current
+stream and can be captured into a graph.  A backward pass that is captured has to be the first use of its leaves'
+gradients on that stream (torch's own rule): take them with `torch.autograd.grad`, or let no eager graph of the same
+leaves live during the capture.  Second derivatives are not available.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from ...cuda import mx
+
+
+def _rows(t):
+    """`t` where its strides are rows of neighbouring columns, else a contiguous copy (an expanded gradient)."""
+    return t if mx.row_stride(t) is not None else t.contiguous()
+
+
+def _check(x, weight=None, bias=None):
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
+        if t.dtype not in mx._TYPES or not t.is_cuda:
+            raise TypeError(f"{name}: expected a float32, bfloat16 or float16 GPU tensor, got {t.dtype} on {t.device}")
+        if t.dtype != x.dtype or t.device != x.device:
+            raise TypeError(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+    if x.dim() < 1:
+        raise ValueError("x: expected at least 1 dimension")
+    if weight is not None and (weight.dim() != 2 or weight.shape[1] != x.shape[-1]):
+        raise ValueError(f"weight {tuple(weight.shape)} does not fit x {tuple(x.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"bias {tuple(bias.shape)} does not fit weight {tuple(weight.shape)}")
+
+
+def _save(x):
+    x = _rows(x)
+    rows, cols = mx.shape2(x)
+    c, s = mx.act8_empty(rows, cols, device=x.device)
+    mx.cu_fn_act8_save_e(x, c, s, sync=False)
+    return c, s
+
+
+def _weight_grads(dy, c, s, weight_like, need_w, need_b):
+    """Gradients of weight and bias from the checkpoint, in the weight's type."""
+    if not need_w:
+        n = dy.shape[-1]
+        return None, (dy.reshape(-1, n).sum(0, dtype=torch.float32).to(dy.dtype) if need_b else None)
+    n, k = weight_like
+    dw = torch.empty(n, k, dtype=torch.float32, device=dy.device)
+    db = torch.empty(n, dtype=torch.float32, device=dy.device) if need_b else None
+    mx.cu_fn_act8_wgrad_e(dw, dy, c, s, DB=db, sync=False)
+    return dw.to(dy.dtype), db.to(dy.dtype) if need_b else None
+
+
+class _Act8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.saved_x = ctx.needs_input_grad[1]
+        ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
+        return torch.nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        weight, *packed = ctx.saved_tensors
+        dy = _rows(dy)
+        dx = dy @ weight if ctx.needs_input_grad[0] else None
+        c, s = packed if ctx.saved_x else (None, None)
+        dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return dx, dw, db
+
+
+class _Act8Act(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, fn):
+        x = _rows(x)
+        rows, cols = mx.shape2(x)
+        c, s = mx.act8_empty(rows, cols, device=x.device)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mx.cu_fn_act8_save_e(x, c, s, Y=y, fn=fn, sync=False)
+        ctx.save_for_backward(c, s)
+        ctx.fn = fn
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        c, s = ctx.saved_tensors
+        dy = _rows(dy)
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        mx.cu_fn_act8_grad_e(dx, dy, c, s, ctx.fn, sync=False)
+        return dx, None
+
+
+class _Mx4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.saved_x = ctx.needs_input_grad[1]
+        ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
+        return Mx4Weight(weight).linear(x, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        weight, *packed = ctx.saved_tensors
+        dy = _rows(dy)
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = Mx4Weight(weight, transpose=True).linear(dy)
+        c, s = packed if ctx.saved_x else (None, None)
+        dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return dx, dw, db
+
+
+def act8_linear(x, weight, bias=None):
+    """torch.nn.functional.linear that keeps x in 8 bits (a quarter of fp32, half of 16 bits) for the weight gradient."""
+    _check(x, weight, bias)
+    return _Act8Linear.apply(x, weight, bias)
+
+
+def act8_act(x, fn):
+    """fn(x) ("gelu": x Phi(x), "silu": x / (1 + e^-x)) that keeps x in 8 bits for its gradient."""
+    _check(x)
+    mx._fn_code(fn, False)
+    return _Act8Act.apply(x, fn)
+
+
+def mx4_linear(x, weight, bias=None):
+    """A linear layer whose products run on 4-bit operands, with gradients; the weight is laid out anew in every pass."""
+    _check(x, weight, bias)
+    return _Mx4Linear.apply(x, weight, bias)
+
+
+class Mx4Weight:
+    """The mx4 codes of a weight [out, in] (of its transpose with ``transpose=True``): 4.25 bits an element."""
+
+    def __init__(self, weight, transpose=False):
+        w = _rows(weight.detach())
+        n, k = w.shape
+        self.shape = (k, n) if transpose else (n, k)
+        self.codes, self.scales = mx.mx4_empty(*self.shape, device=w.device)
+        mx.cu_fn_mx4_quantize_e(w, self.codes, self.scales, transpose=transpose, sync=False)
+
+    def linear(self, x, bias=None):
+        """mx4(x) W^T (+ bias), [..., in] -> [..., out]; for use without gradients."""
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+            raise RuntimeError("Mx4Weight.linear has no gradient: use mx4_linear, or torch.no_grad()")
+        if x.shape[-1] != self.shape[1]:
+            raise ValueError(f"x {tuple(x.shape)} does not fit the weight {self.shape}")
+        x = _rows(x)
+        y = torch.empty(*x.shape[:-1], self.shape[0], dtype=x.dtype, device=x.device)
+        mx.cu_fn_mx4_linear_e(y, x, self.codes, self.scales, bias=bias, sync=False)
+        return y
