@@ -36,6 +36,9 @@ constexpr int kStep = NKMX_STEP;        // columns of a step
 constexpr int kStepBytes4 = kStep / 2;  // its mx4 codes
 constexpr uint32_t kInfBits = 0x7F800000u;
 
+// On a lambda: arrays that it captures stay in registers only where it is inlined.
+#define NKMX_INLINE __attribute__((always_inline))
+
 // n / d for 32-bit n: one high product with a 64-bit reciprocal (exact: the error of the reciprocal, below
 // 2^-64 relative to 1/d, times n < 2^32 stays below 1/d).
 struct FastDiv {
@@ -591,15 +594,40 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t row_tiles, uint32_t
 // ---------------------------------------------------------------- mx4 product, tiles
 //
 // A workgroup computes TM x TN of y in waves of WM x WN (32 x 32 x 64 matrix instructions: lane l holds row
-// l % 32 and one block of 32 columns); the steps of k go through two LDS buffers, loaded into registers one
-// step ahead.  LDS holds a tile row as 64 bytes = 4 slots of 16; slot s of row r lies at s ^ swizzle4(r), so
-// that rows a bank period apart do not meet.  The two half-steps of a lane are blocks 2g and 2g + 1 (g =
-// l / 32): any assignment of blocks to instructions is right as long as both operands agree, and in this one a
-// lane's two scale bytes are neighbours: one 16-bit LDS read, selected by the instruction's own byte index.
+// l % 32 and one block of 32 columns).  k goes by in stages of 256 columns = 128 bytes = one cache line a row,
+// through two LDS buffers that buffer loads fill directly, one stage ahead.  LDS holds a tile row as 8 slots of
+// 16 bytes; slot s of row r lies at s ^ swizzle8(r), so that the 16 rows that are read together do not meet; a
+// load writes LDS in lane order, so the lanes' addresses carry the exchange.  The buffer's extent ends the rows: a
+// row past the matrix is not read, and its results are not stored.
 
-__device__ __forceinline__ uint32_t swizzle4(uint32_t row)
+constexpr int kSpan = 4;  // steps whose scales are loaded at a time
+
+// LDS serves 16 lanes' 16 bytes at a time over 256 bytes of banks: of 16 rows at 128 bytes each, those of one
+// parity share their banks and need 8 slots of their own.
+__device__ __forceinline__ uint32_t swizzle8(uint32_t row) { return (row & 6u) | ((row ^ (row >> 3)) & 1u); }
+
+// The words of a raw buffer's descriptor.
+__device__ __forceinline__ u32x4 buffer_of(const void* p, uint32_t bytes)
 {
-    return ((row >> 1) & 2u) | (((row >> 1) ^ (row >> 3)) & 1u);
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, bytes, 0x00027000u};
+}
+
+// 64 lanes load 16 bytes each from `at` of the buffer to LDS from `lds` on, in lane order; what lies past the
+// buffer's end is not read (the whole offset is in the lane's register: only that is checked).  Written as
+// assembly because the compiler makes every LDS read wait for every such load it knows of, also one into the
+// other buffer; nothing comes back in registers.  The caller waits (arrived()) before the barrier that hands
+// the data on.  The nop is the wait state between a write of M0 and a load to LDS.
+__device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t at, const void* lds)
+{
+    const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(base), "v"(at), "s"(buffer) : "memory");
+}
+// This wave's loads to LDS have arrived, and everybody's; what was read before is free to be overwritten.
+__device__ __forceinline__ void arrived()
+{
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 template <typename T, int TM, int TN, int WM, int WN>
@@ -607,104 +635,194 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
     T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb, const T* bias,
     uint32_t m, uint32_t n, uint32_t steps, uint32_t row_tiles, uint32_t col_tiles)
 {
-    constexpr int NT = 64 * (TM / WM) * (TN / WN), WAVES_N = TN / WN;
+    constexpr int WAVES = (TM / WM) * (TN / WN), WAVES_N = TN / WN;
     constexpr int FM = WM / 32, FN = WN / 32;
-    constexpr int CHUNKS = (TM + TN) * 4 / NT;   // 16-byte pieces a thread moves per step
-    constexpr int SCALES = (TM + TN + NT - 1) / NT;
-    static_assert((TM * 4) % NT == 0 && (TN * 4) % NT == 0, "each thread's pieces belong to one operand");
-    __shared__ u32x4 image[2][(TM + TN) * 4];
-    __shared__ uint32_t bytes[2][TM + TN];
+    static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && WAVES % 2 == 0, "whole rounds of row groups");
+    __shared__ u32x4 image[2][(TM + TN) * 8];
+    __shared__ uint32_t bytes[2][(TM + TN) * kSpan];
 
     uint32_t tr, tc;
     tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
     const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
+    const uint32_t stages = (steps + 1) / 2;
+    const uint32_t pitch = steps * kStepBytes4, pitch_s = steps * 4;
+    const uint32_t rows_a = min((uint32_t)TM, m - tr * TM), rows_b = min((uint32_t)TN, n - tc * TN);
+    const u32x4 buf_a = buffer_of(ca + (uint64_t)tr * TM * pitch, rows_a * pitch);
+    const u32x4 buf_b = buffer_of(cb + (uint64_t)tc * TN * pitch, rows_b * pitch);
+    const u32x4 buf_sa = buffer_of(sa + (uint64_t)tr * TM * pitch_s, rows_a * pitch_s);
+    const u32x4 buf_sb = buffer_of(sb + (uint64_t)tc * TN * pitch_s, rows_b * pitch_s);
+    // 8 rows a load; a wave's row groups are all even or all odd ones
+    const uint32_t at = (lane >> 3) * pitch + (((lane & 7) ^ swizzle8((wave & 1) * 8 + (lane >> 3))) << 4);
+    const uint32_t at_s = lane * pitch_s;  // 64 rows a load
 
-    // rows past the end read the last row: their results are not stored
-    const u32x4* from[CHUNKS];
-    const uint32_t* from_s[SCALES];
+    const auto fetch = [&](uint32_t stage, int buf) {
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-        const uint32_t c = tid + i * NT, row = c >> 2, slot = c & 3;
-        const bool is_a = row < TM;
-        const uint32_t at = is_a ? min(tr * TM + row, m - 1) : min(tc * TN + (row - TM), n - 1);
-        from[i] = reinterpret_cast<const u32x4*>(is_a ? ca : cb) + (uint64_t)at * steps * 4 + (slot ^ swizzle4(row));
-    }
+        for (int i = 0; i < TM / 8 / WAVES; ++i) {
+            const int group = i * WAVES + wave;
+            load_to_lds(buf_a, at + (group * 8 * pitch + stage * 128), &image[buf][group * 64]);
+        }
 #pragma unroll
-    for (int i = 0; i < SCALES; ++i) {
-        const uint32_t row = min((uint32_t)(tid + i * NT), (uint32_t)(TM + TN - 1));
-        const bool is_a = row < TM;
-        const uint32_t at = is_a ? min(tr * TM + row, m - 1) : min(tc * TN + (row - TM), n - 1);
-        from_s[i] = reinterpret_cast<const uint32_t*>(is_a ? sa : sb) + (uint64_t)at * steps;
-    }
-    u32x4 next[CHUNKS];
-    uint32_t next_s[SCALES];
-    auto fetch = [&](uint32_t s) {
+        for (int i = 0; i < TN / 8 / WAVES; ++i) {
+            const int group = i * WAVES + wave;
+            load_to_lds(buf_b, at + (group * 8 * pitch + stage * 128), &image[buf][TM * 8 + group * 64]);
+        }
+        // Scales of two stages at a time: 16 bytes a row, each in a cache line of its own, whose look-up is what such a
+        // load costs
+        if ((stage & 1) == 0) {
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) next[i] = from[i][(uint64_t)s * 4];
-#pragma unroll
-        for (int i = 0; i < SCALES; ++i) next_s[i] = from_s[i][s];
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) image[buf][tid + i * NT] = next[i];
-#pragma unroll
-        for (int i = 0; i < SCALES; ++i)
-            if (tid + i * NT < TM + TN) bytes[buf][tid + i * NT] = next_s[i];
+            for (int i = 0; i < ((TM + TN) / 64 + WAVES - 1) / WAVES; ++i) {
+                const int group = i * WAVES + wave;
+                uint32_t* to = &bytes[(stage >> 1) & 1][group * 64 * kSpan];
+                if (group < TM / 64)
+                    load_to_lds(buf_sa, at_s + (group * 64 * pitch_s + stage * 8), to);
+                else if (group < (TM + TN) / 64)
+                    load_to_lds(buf_sb, at_s + ((group - TM / 64) * 64 * pitch_s + stage * 8), to);
+            }
+        }
     };
 
     f32x16 acc[FM][FN] = {};
-    fetch(0);
-    put(0);
-    __syncthreads();
-    const uint32_t sw = swizzle4(r);  // tile rows of a fragment start at multiples of 32
-    for (uint32_t s = 0; s < steps; ++s) {
-        const int buf = s & 1;
-        if (s + 1 < steps) fetch(s + 1);
-        uint32_t ea[FM], eb[FN];
-        const uint16_t* half = reinterpret_cast<const uint16_t*>(bytes[buf]);
+    // Operands of instruction h of a stage: lane g takes block h of the stage's step g (any assignment of blocks
+    // to instructions is right as long as both operands agree), so that its four scale bytes are one word that the
+    // instructions index themselves.
+    struct Operands {
+        u32x4 a[FM], b[FN];
+    };
+    const auto take = [&](Operands& o, int buf, int h) {
+        const uint32_t slot = (4 * g + h) ^ swizzle8(r);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) ea[i] = half[(wm + 32 * i + r) * 2 + g];
+        for (int j = 0; j < FN; ++j) o.b[j] = image[buf][(TM + wn + 32 * j + r) * 8 + slot];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) eb[j] = half[(TM + wn + 32 * j + r) * 2 + g];
+        for (int i = 0; i < FM; ++i) o.a[i] = image[buf][(wm + 32 * i + r) * 8 + slot];
+    };
+    struct Scales {
+        int a[FM], b[FN];
+    };
+    const auto take_scales = [&](Scales& e, uint32_t stage) {
+        const uint32_t* from = bytes[(stage >> 1) & 1] + (stage & 1) * 2 + g;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            i32x8 a[FM], b[FN];
-            const uint32_t slot = (2 * g + h) ^ sw;
+        for (int i = 0; i < FM; ++i) e.a[i] = from[(wm + 32 * i + r) * kSpan];
 #pragma unroll
-            for (int i = 0; i < FM; ++i) a[i] = operand4(image[buf][(wm + 32 * i + r) * 4 + slot]);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) b[j] = operand4(image[buf][(TM + wn + 32 * j + r) * 4 + slot]);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    if (h == 0)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 0,
-                                                                                   (int)ea[i], 0, (int)eb[j]);
-                    else
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 1,
-                                                                                   (int)ea[i], 1, (int)eb[j]);
-                }
-        }
-        if (s + 1 < steps) put(buf ^ 1);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const uint32_t col = tc * TN + wn + 32 * j + r;
-        const float add = bias && col < n ? number(bias[col]) : 0.0f;
+        for (int j = 0; j < FN; ++j) e.b[j] = from[(TM + wn + 32 * j + r) * kSpan];
+    };
+    const auto multiply = [&](const Operands& o, const Scales& e, auto index) {
+        constexpr int h = decltype(index)::value;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const uint32_t row = tr * TM + wm + 32 * i + 8 * (e / 4) + 4 * g + e % 4;
-                if (row < m && col < n) {
-                    float v = acc[i][j][e];
-                    if (bias) v += add;
-                    y[row * ldy + col] = (T)v;
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand4(o.a[i]), operand4(o.b[j]), acc[i][j],
+                                                                           4, 4, h, e.a[i], h, e.b[j]);
+    };
+    // While the instructions of one operand set run, the next set is read, a read after every instruction from the
+    // first on: left alone the compiler reads late and waits, or reads a whole stage at once, which does not fit
+    // the registers.
+    const auto interleave = [](auto reads) {
+        constexpr int kMfma = 0x008, kLdsRead = 0x100, n = decltype(reads)::value, each = (n + FM * FN - 1) / (FM * FN);
+#pragma unroll
+        for (int i = 0; i < FM * FN; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kLdsRead, each, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    typedef std::integral_constant<int, FM + FN> One;
+    typedef std::integral_constant<int, 2 * (FM + FN)> Two;
+
+    Operands o, p;
+    Scales e, f;
+    const auto one_stage = [&](uint32_t s, const Scales& now, Scales& next) {
+        const int buf = s & 1;
+        if (s + 1 < stages) fetch(s + 1, buf ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        take(p, buf, 1);
+        multiply(o, now, std::integral_constant<int, 0>{});
+        interleave(One{});
+        take(o, buf, 2);
+        multiply(p, now, std::integral_constant<int, 1>{});
+        interleave(One{});
+        take(p, buf, 3);
+        multiply(o, now, std::integral_constant<int, 2>{});
+        interleave(One{});
+        // this stage has been read; what follows reads the next one while the last instructions run (after the last
+        // stage: what is there, unused)
+        arrived();
+        take(o, buf ^ 1, 0);
+        take_scales(next, s + 1);
+        multiply(p, now, std::integral_constant<int, 3>{});
+        interleave(Two{});
+    };
+    const uint32_t whole = steps / 2;
+    fetch(0, 0);
+    arrived();
+    take(o, 0, 0);
+    take_scales(e, 0);
+    for (uint32_t s = 0; s < whole; ++s) {
+        one_stage(s, e, f);
+        e = f;
+    }
+    if (steps & 1) {  // half a stage: the lanes of its second step take part with zeros
+        const auto rest = [&](auto index) {
+            if (decltype(index)::value) take(o, whole & 1, decltype(index)::value);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                if (g) o.a[i] = u32x4{0u, 0u, 0u, 0u};
+            }
+            multiply(o, e, index);
+        };
+#pragma unroll
+        for (int i = 0; i < FM; ++i) e.a[i] = g ? 0 : e.a[i];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) e.b[j] = g ? 0 : e.b[j];
+        rest(std::integral_constant<int, 0>{});
+        rest(std::integral_constant<int, 1>{});
+        rest(std::integral_constant<int, 2>{});
+        rest(std::integral_constant<int, 3>{});
+    }
+    arrived();
+
+    // The results cross LDS, 32 rows of the wave at a time, so that they leave in 16-byte pieces of whole lines.
+    constexpr int kRowBytes = WN * 4 + 32, E = 16 / (int)sizeof(T), kPerRow = WN / E, kRows = 64 / kPerRow;
+    static_assert(WAVES * 32 * kRowBytes <= (int)sizeof(image), "a wave's rows in LDS");
+    char* mine = reinterpret_cast<char*>(image) + wave * 32 * kRowBytes;
+    const uint32_t col = tc * TN + wn + (lane % kPerRow) * E;
+    const int64_t live = (int64_t)n - (int64_t)col;
+    float add[E];
+#pragma unroll
+    for (int c = 0; c < E; ++c) add[c] = bias && c < live ? number(bias[col + c]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                *reinterpret_cast<float*>(mine + (8 * (v / 4) + 4 * g + v % 4) * kRowBytes + (32 * j + r) * 4) = acc[i][j][v];
+#pragma unroll
+        for (int k = 0; k < 32 / kRows; ++k) {
+            const int at_row = k * kRows + lane / kPerRow;
+            const uint32_t row = tr * TM + wm + 32 * i + at_row;
+            const float* from = reinterpret_cast<const float*>(mine + at_row * kRowBytes) + (lane % kPerRow) * E;
+            typename Pack<T, E>::vec out;
+#pragma unroll
+            for (int c = 0; c < E; c += 4) {
+                const f32x4 four = *reinterpret_cast<const f32x4*>(from + c);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) out[c + u] = (T)(bias ? four[u] + add[c + u] : four[u]);
+            }
+            // cached stores: y is read next, and lines shared with a neighbouring tile meet in L2
+            if (row < m) {
+                T* to = y + row * ldy + col;
+                if (live >= E) {
+                    *reinterpret_cast<typename Pack<T, E>::loose*>(to) = out;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < E; ++c)
+                        if (c < live) to[c] = out[c];
                 }
             }
+        }
     }
 }
 
@@ -738,11 +856,11 @@ __device__ __forceinline__ uint32_t lower_halves(uint32_t first, uint32_t second
     return __builtin_amdgcn_perm(second, first, 0x05040100u);
 }
 
-// What is left of v after its upper 8 significant bits.  An infinity leaves nothing, a NaN a NaN.
+// The upper 8 significant bits of v, and what they leave: an infinity leaves nothing, a NaN a NaN.
+__device__ __forceinline__ float upper_part(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
 __device__ __forceinline__ float rest_of(float v)
 {
-    const float left = v - __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
-    return magnitude(v) == kInfBits ? 0.0f : left;
+    return magnitude(v) == kInfBits ? 0.0f : v - upper_part(v);
 }
 
 template <typename T>
@@ -754,6 +872,78 @@ struct Parts<f16> { static constexpr int count = 2; };
 template <>
 struct Parts<float> { static constexpr int count = 3; };
 
+// f(0), f(1) .. f(N - 1) with the numbers as constants.
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f)
+{
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// Up to this token every load of a tile stays inside the matrices: a row's end runs on into the next rows, whose
+// numbers end in results that are not stored.  `end_d`, `end_x`: the tile's last column + 1 in dy and in the codes.
+__device__ __forceinline__ uint32_t safe_tokens(uint32_t t_rows, uint32_t n, uint32_t end_d, uint64_t lddy, uint32_t pitch,
+                                                uint32_t end_x)
+{
+    const uint32_t over_d = end_d > n ? end_d - n : 0, over_x = end_x > pitch ? end_x - pitch : 0;
+    const uint32_t ld = (uint32_t)max(lddy, (uint64_t)1);
+    const uint32_t rows = max((over_d + ld - 1) / ld, over_x ? (over_x + pitch - 1) / max(pitch, 1u) : 0u);
+    return pitch && t_rows > rows ? t_rows - rows : 0;
+}
+
+// The scales of a unit's 8 tokens from one scale byte a lane: lane % 8 has that token's, and the 8 lanes around it have
+// the same 32 columns.
+__device__ __forceinline__ void spread_scales(uint32_t byte, float (&scale)[8])
+{
+    const int v = __float_as_int(scale_value(byte));
+    scale[0] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 0 << 5));
+    scale[1] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 1 << 5));
+    scale[2] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 2 << 5));
+    scale[3] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 3 << 5));
+    scale[4] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 4 << 5));
+    scale[5] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 5 << 5));
+    scale[6] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 6 << 5));
+    scale[7] = __int_as_float(__builtin_amdgcn_ds_swizzle(v, 0x18 | 7 << 5));
+}
+
+// Column j of a unit's codes as 8 tokens in bf16.
+__device__ __forceinline__ u32x4 eight_tokens(const uint32_t (&q)[8], const float (&scale)[8], int j)
+{
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = (float)(int8_t)(q[2 * i] >> (8 * j)) * scale[2 * i];
+        const float b = (float)(int8_t)(q[2 * i + 1] >> (8 * j)) * scale[2 * i + 1];
+        w[i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)a, (bf16)b});
+    }
+    return w;
+}
+
+// A wave's part of dw.
+template <int FN, int FK>
+__device__ __forceinline__ void store_gradient(const f32x16 (&acc)[FN][FK], float* dw, uint64_t lddw, uint32_t row0,
+                                               uint32_t col0, uint32_t n, uint32_t k, uint32_t accumulate, int r, int g)
+{
+#pragma unroll
+    for (int j = 0; j < FK; ++j) {
+        const uint32_t col = col0 + 32 * j + r;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const uint32_t row = row0 + 32 * i + 8 * (v / 4) + 4 * g + v % 4;
+                if (row < n && col < k) {
+                    float* p = dw + row * lddw + col;
+                    *p = accumulate ? *p + acc[i][j][v] : acc[i][j][v];
+                }
+            }
+    }
+}
+
 template <typename T, int TN, int TK, int WN, int WK, int BT>
 __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
     float* dw, uint64_t lddw, float* db, const T* dy, uint64_t lddy, const uint8_t* codes, const uint8_t* scales,
@@ -761,179 +951,224 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
     uint32_t stages_each, uint32_t accumulate, uint64_t part_stride, uint64_t part_stride_db)
 {
     constexpr int NT = 64 * (TN / WN) * (TK / WK), WAVES_K = TK / WK, P = Parts<T>::count;
-    constexpr int FN = WN / 32, FK = WK / 32, SLOTS = BT / 8;
-    constexpr int UD = SLOTS * (TN / 4), UX = SLOTS * (TK / 4);  // units of 8 tokens x 4 columns
-    constexpr bool BOTH = UD >= NT;                              // a thread has a unit of each, or one of one
-    static_assert(BOTH ? (UD == NT && UX == NT) : (UD + UX <= NT && UD % 64 == 0), "units and threads");
+    constexpr int FN = WN / 32, FK = WK / 32, SLOTS = BT / 8, GROUPS = BT / 16;
+    constexpr int CD = TN / 4, CX = TK / 4;             // groups of 4 columns
+    constexpr int UD = SLOTS * CD, UX = SLOTS * CX;     // units of 8 tokens x 4 columns
+    constexpr bool BOTH = UD >= NT;                     // a thread has a unit of each, or one of one
+    constexpr int XW = BOTH ? 0 : UD / 64;              // first wave with units of x
+    static_assert(BOTH ? (UD == NT && UX == NT) : (UD + UX == NT && UD % 64 == 0), "units and threads");
     __shared__ u32x4 left[2][P][TN * SLOTS];
     __shared__ u32x4 right[2][TK * SLOTS];
 
     uint32_t tr, tc;
     tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
     const int wn = (wave / WAVES_K) * WN, wk = (wave % WAVES_K) * WK;
     const uint32_t stages = (t_rows + BT - 1) / BT;
     const uint32_t first = blockIdx.y * stages_each, last = min(stages, first + stages_each);
 
-    const bool has_d = BOTH || tid < UD, has_x = BOTH || (tid >= UD && tid < UD + UX);
-    const int ud = tid, ux = BOTH ? tid : tid - UD;
-    const int d_slot = ud / (TN / 4), d_col = (ud % (TN / 4)) * 4;
-    const int x_slot = ux / (TK / 4), x_col = (ux % (TK / 4)) * 4;
-    const int64_t live_d = (int64_t)n - (int64_t)(tr * TN + d_col);
-    const uint32_t col_x = tc * TK + x_col;
-    const bool live_x = has_x && col_x < steps * kStep;
-    const bool sums_dy = db != nullptr && tc == 0 && has_d;
+    // slot (8 tokens) of a unit: the wave's first one and the lane's from there; columns
+    const int d_slot0 = wave * 64 / CD, d_slot = d_slot0 + lane / CD, d_col = (lane % CD) * 4;
+    const int x_slot0 = (wave - XW) * 64 / CX, x_slot = x_slot0 + lane / CX, x_col = (lane % CX) * 4;
+    const uint32_t pitch = steps * kStep, pitch_s = steps * 4, col_x = tc * TK + x_col;
+    const uint32_t safe = safe_tokens(t_rows, n, (tr + 1) * TN, lddy, pitch, (tc + 1) * TK);
+    const uint32_t at_d = (uint32_t)(lane / CD) * 8 * (uint32_t)lddy * sizeof(T) + d_col * sizeof(T);
+    const uint32_t at_x = (lane / CX) * 8 * pitch + x_col;
+    const uint32_t at_s = ((lane / CX) * 8 + (lane & 7)) * pitch_s + x_col / 32;
 
+    // Stages up to `safe` load whole tiles; the others element by element, with zeros past the ends.
     typename Pack<T, 4>::vec d[8];
-    uint32_t q[8];
-    uint8_t e[8];
-    auto fetch = [&](uint32_t stage) {
-        if (has_d) {
-            const uint32_t t0 = stage * BT + d_slot * 8;
-            const T* p = dy + (uint64_t)t0 * lddy + tr * TN + d_col;
+    const auto fetch_d = [&](uint32_t stage) NKMX_INLINE {
+        const char* p = reinterpret_cast<const char*>(dy + (uint64_t)(stage * BT + d_slot0 * 8) * lddy + tr * TN);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                d[i] = typename Pack<T, 4>::vec{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
-                if (t0 + i < t_rows && live_d > 0) {
-                    if (live_d >= 4) {
-                        d[i] = *reinterpret_cast<const typename Pack<T, 4>::loose*>(p + (uint64_t)i * lddy);
-                    } else {
+        for (int i = 0; i < 8; ++i)
+            d[i] = *reinterpret_cast<const typename Pack<T, 4>::loose*>(p + (uint64_t)i * lddy * sizeof(T) + at_d);
+    };
+    const auto copy_d = [&](uint32_t stage) NKMX_INLINE {
+        const uint32_t t = stage * BT + d_slot * 8;
+        const int64_t live = (int64_t)n - (int64_t)(tr * TN + d_col);
+        const T* p = dy + (uint64_t)t * lddy + tr * TN + d_col;
 #pragma unroll
-                        for (int j = 0; j < 3; ++j)
-                            if (j < live_d) d[i][j] = p[(uint64_t)i * lddy + j];
-                    }
-                }
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                d[i][j] = (T)0.0f;
+                if (t + i < t_rows && j < live) d[i][j] = p[(uint64_t)i * lddy + j];
             }
-        }
-        if (has_x) {
-            const uint32_t t0 = stage * BT + x_slot * 8;
-            const uint8_t* p = codes + (uint64_t)t0 * steps * kStep + col_x;
-            const uint8_t* ps = scales + (uint64_t)t0 * steps * 4 + col_x / 32;
+    };
+    uint32_t q[8], e;  // codes; scale byte of the unit's token lane % 8
+    const auto fetch_x = [&](uint32_t stage) NKMX_INLINE {
+        const uint32_t t = stage * BT + x_slot0 * 8;
+        const uint8_t* p = codes + (uint64_t)t * pitch + tc * TK;
+        e = (scales + (uint64_t)t * pitch_s + tc * (TK / 32))[at_s];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[i] = 0u;
-                e[i] = 0;
-                if (live_x && t0 + i < t_rows) {
-                    q[i] = *reinterpret_cast<const uint32_t*>(p + (uint64_t)i * steps * kStep);
-                    e[i] = ps[(uint64_t)i * steps * 4];
-                }
-            }
+        for (int i = 0; i < 8; ++i) q[i] = *reinterpret_cast<const uint32_t*>(p + (uint64_t)i * pitch + at_x);
+    };
+    const auto copy_x = [&](uint32_t stage) NKMX_INLINE {
+        const uint32_t t = stage * BT + x_slot * 8;
+        const bool live = col_x < pitch;
+        e = 0;
+        if (live && t + (lane & 7) < t_rows) e = scales[(uint64_t)(t + (lane & 7)) * pitch_s + col_x / 32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            q[i] = 0u;
+            if (live && t + i < t_rows) q[i] = *reinterpret_cast<const uint32_t*>(codes + (uint64_t)(t + i) * pitch + col_x);
         }
     };
     float sum_dy[4] = {};
-    auto put = [&](int buf) {
-        if (has_d) {
+    // Column j of the unit into LDS.
+    const auto put_d = [&](int buf, int j, auto sums) NKMX_INLINE {
+        const uint32_t c = d_col + j, at = c * SLOTS + (d_slot ^ swizzle_t<SLOTS>(c));
+        if constexpr (P == 1) {
+            u32x4 w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t c = d_col + j, at = c * SLOTS + (d_slot ^ swizzle_t<SLOTS>(c));
-                if (sums_dy) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum_dy[j] += number(d[i][j]);
-                }
-                if constexpr (P == 1) {
-                    u32x4 w;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t a = __builtin_bit_cast(u32x2, d[2 * i])[j / 2];
-                        const uint32_t b = __builtin_bit_cast(u32x2, d[2 * i + 1])[j / 2];
-                        w[i] = j % 2 ? upper_halves(a, b) : lower_halves(a, b);
-                    }
-                    left[buf][0][at] = w;
-                } else {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = number(d[i][j]);
-#pragma unroll
-                    for (int part = 0; part < P; ++part) {
-                        u32x4 w;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            w[i] = upper_halves(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
-                        left[buf][part][at] = w;
-                        if (part + 1 < P) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) v[i] = rest_of(v[i]);
-                        }
-                    }
-                }
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a = __builtin_bit_cast(u32x2, d[2 * i])[j / 2];
+                const uint32_t b = __builtin_bit_cast(u32x2, d[2 * i + 1])[j / 2];
+                const uint32_t two = j % 2 ? upper_halves(a, b) : lower_halves(a, b);
+                w[i] = two;
+                if constexpr (decltype(sums)::value)
+                    sum_dy[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two),
+                                                                bf16x2{(bf16)1.0f, (bf16)1.0f}, sum_dy[j], false);
             }
-        }
-        if (has_x) {
-            float s[8], zero[8];
-            uint32_t u[8];
+            left[buf][0][at] = w;
+        } else {
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s[i] = scale_value(e[i]);
-                zero[i] = -128.0f * s[i];
-                u[i] = q[i] ^ 0x80808080u;  // q + 128 as an unsigned byte: one conversion each
+            for (int i = 0; i < 8; ++i) v[i] = number(d[i][j]);
+            if constexpr (decltype(sums)::value) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum_dy[j] += v[i];
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t c = x_col + j;
+            for (int part = 0; part < P; ++part) {
                 u32x4 w;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = fmaf((float)((u[2 * i] >> (8 * j)) & 255u), s[2 * i], zero[2 * i]);
-                    const float b = fmaf((float)((u[2 * i + 1] >> (8 * j)) & 255u), s[2 * i + 1], zero[2 * i + 1]);
-                    w[i] = __builtin_bit_cast(uint32_t, bf16x2{(bf16)a, (bf16)b});
+                for (int i = 0; i < 4; ++i) w[i] = upper_halves(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]));
+                left[buf][part][at] = w;
+                if (part + 1 < P) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = part == 0 ? rest_of(v[i]) : v[i] - upper_part(v[i]);
                 }
-                right[buf][c * SLOTS + (x_slot ^ swizzle_t<SLOTS>(c))] = w;
             }
         }
     };
+    float scale[8];
+    const auto put_x = [&](int buf, int j) NKMX_INLINE {
+        const uint32_t c = x_col + j;
+        right[buf][c * SLOTS + (x_slot ^ swizzle_t<SLOTS>(c))] = eight_tokens(q, scale, j);
+    };
 
     f32x16 acc[FN][FK] = {};
-    if (first < last) {
-        fetch(first);
-        put(0);
-    }
-    __syncthreads();
-    for (uint32_t s = first; s < last; ++s) {
-        const int buf = (s - first) & 1;
-        if (s + 1 < last) fetch(s + 1);
+    bf16x8 a[FN], b[2][FK];
+    const auto take_b = [&](int buf, int h) NKMX_INLINE {
 #pragma unroll
-        for (int h = 0; h < BT / 16; ++h) {
-            bf16x8 b[FK];
-#pragma unroll
-            for (int j = 0; j < FK; ++j) {
-                const uint32_t c = wk + 32 * j + r;
-                b[j] = __builtin_bit_cast(bf16x8, right[buf][c * SLOTS + ((2 * h + g) ^ swizzle_t<SLOTS>(c))]);
-            }
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const uint32_t c = wn + 32 * i + r;
-#pragma unroll
-                for (int part = P - 1; part >= 0; --part) {  // smallest first
-                    const bf16x8 a =
-                        __builtin_bit_cast(bf16x8, left[buf][part][c * SLOTS + ((2 * h + g) ^ swizzle_t<SLOTS>(c))]);
-#pragma unroll
-                    for (int j = 0; j < FK; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
-                }
-            }
+        for (int j = 0; j < FK; ++j) {
+            const uint32_t c = wk + 32 * j + r;
+            b[h & 1][j] = __builtin_bit_cast(bf16x8, right[buf][c * SLOTS + ((2 * h + g) ^ swizzle_t<SLOTS>(c))]);
         }
-        if (s + 1 < last) put(buf ^ 1);
-        __syncthreads();
+    };
+    const auto take_a = [&](int buf, int u, int i) NKMX_INLINE {  // for step u: 16 tokens u / P, the smallest part first
+        const uint32_t c = wn + 32 * i + r;
+        a[i] = __builtin_bit_cast(bf16x8, left[buf][P - 1 - u % P][c * SLOTS + ((2 * (u / P) + g) ^ swizzle_t<SLOTS>(c))]);
+    };
+    // A step: one part of 16 tokens.  An operand is read for the next step as soon as it has been used; those reads and
+    // the instructions of what `work` adds go between the matrix instructions.
+    constexpr int STEPS = GROUPS * P;
+    const auto step = [&](int buf, auto index, auto work) NKMX_INLINE {
+        constexpr int u = decltype(index)::value;
+        if constexpr (u + 1 < STEPS && (u + 1) % P == 0) take_b(buf, (u + 1) / P);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+#pragma unroll
+            for (int j = 0; j < FK; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[(u / P) & 1][j], acc[i][j], 0, 0, 0);
+            if constexpr (u + 1 < STEPS) take_a(buf, u + 1, i);
+        }
+        work();
+#pragma unroll
+        for (int z = 0; z < FN * FK; ++z) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // others
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // an LDS write
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // A stage; with MORE the next one is loaded at its beginning and turned into the other buffer over its last steps, a
+    // column of the units at a time.  D, X: whether this wave has units of dy, of x.
+    const auto run = [&](auto sums, auto has_d, auto has_x) NKMX_INLINE {
+        constexpr bool D = decltype(has_d)::value, X = decltype(has_x)::value;
+        const auto put = [&](int buf, int j) NKMX_INLINE {
+            if constexpr (D) put_d(buf, j, sums);
+            if constexpr (X) put_x(buf, j);
+        };
+        const auto stage = [&](uint32_t s, int buf, auto more) NKMX_INLINE {
+            constexpr bool MORE = decltype(more)::value;
+            if constexpr (MORE) {
+                if constexpr (D) fetch_d(s + 1);
+                if constexpr (X) fetch_x(s + 1);
+            }
+            take_b(buf, 0);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) take_a(buf, 0, i);
+            __builtin_amdgcn_sched_barrier(0);
+            each<STEPS>([&](auto index) NKMX_INLINE {
+                step(buf, index, [&]() NKMX_INLINE {
+                    if constexpr (MORE) {
+                        constexpr int u = decltype(index)::value, begin = STEPS > 4 ? STEPS - 4 : 1;
+                        if (X && u == begin) spread_scales(e, scale);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (min(begin + j, STEPS - 1) == u) put(buf ^ 1, j);
+                    }
+                });
+            });
+            __syncthreads();
+        };
+        const uint32_t fast = max(first, min(last, safe / BT));  // stages of whole tiles
+        if (first < fast) {
+            if constexpr (D) fetch_d(first);
+            if constexpr (X) {
+                fetch_x(first);
+                spread_scales(e, scale);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put(0, j);
+            __syncthreads();
+            int buf = 0;
+            for (uint32_t s = first; s + 1 < fast; ++s, buf ^= 1) stage(s, buf, std::true_type{});
+            stage(fast - 1, buf, std::false_type{});
+        }
+#pragma unroll 1
+        for (uint32_t s = fast; s < last; ++s) {  // the last tokens
+            if constexpr (D) copy_d(s);
+            if constexpr (X) {
+                copy_x(s);
+                spread_scales(e, scale);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put(0, j);
+            __syncthreads();
+            stage(s, 0, std::false_type{});
+        }
+    };
+    const auto with_sums = [&](auto has_d, auto has_x) NKMX_INLINE {
+        if (db != nullptr && tc == 0) run(std::true_type{}, has_d, has_x);
+        else run(std::false_type{}, has_d, has_x);
+    };
+    if constexpr (BOTH) {
+        with_sums(std::true_type{}, std::true_type{});
+    } else {  // (both sides meet the same barriers)
+        if (wave < XW) with_sums(std::true_type{}, std::false_type{});
+        else run(std::false_type{}, std::false_type{}, std::true_type{});
     }
 
-    float* out = dw + blockIdx.y * part_stride;
-#pragma unroll
-    for (int j = 0; j < FK; ++j) {
-        const uint32_t col = tc * TK + wk + 32 * j + r;
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const uint32_t row = tr * TN + wn + 32 * i + 8 * (v / 4) + 4 * g + v % 4;
-                if (row < n && col < k) {
-                    float* p = out + row * lddw + col;
-                    *p = accumulate ? *p + acc[i][j][v] : acc[i][j][v];
-                }
-            }
-    }
+    store_gradient<FN, FK>(acc, dw + blockIdx.y * part_stride, lddw, tr * TN + wn, tc * TK + wk, n, k, accumulate, r, g);
     if (db != nullptr && tc == 0) {  // the token groups' sums of a column, joined in order
         float* part = reinterpret_cast<float*>(&right[0][0]);
-        if (has_d) {
+        if (BOTH || wave < XW) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) part[d_slot * TN + d_col + j] = sum_dy[j];
         }
@@ -945,6 +1180,258 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
             float* p = db + blockIdx.y * part_stride_db + tr * TN + tid;
             *p = accumulate ? *p + s : s;
         }
+    }
+}
+
+// The same for bf16 dy on 4-byte boundaries, where nothing has to be cut: dy goes to LDS as it lies in memory, a
+// token's columns in a row, by loads that need no registers, and the turn is made by the transposing LDS reads
+// (16 lanes read 4 tokens x 16 columns and get 4 tokens of one column each).  A row is TN / 32 pieces of 64 bytes; piece
+// c of token t lies at c ^ (t & 3), so that the four tokens that are read together do not meet in the banks.
+//
+// Order of a stage, whose loads count against each other: the codes of the stage after the next are loaded when those
+// of the next one have arrived, the next stage's dy just before them; at the end only the codes may still be on
+// their way.
+template <int TN, int TK, int WN, int WK>
+__global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_kernel(
+    float* dw, uint64_t lddw, float* db, const bf16* dy, uint64_t lddy, const uint8_t* codes, const uint8_t* scales,
+    uint32_t t_rows, uint32_t n, uint32_t k, uint32_t steps, uint32_t row_tiles, uint32_t col_tiles,
+    uint32_t stages_each, uint32_t accumulate, uint64_t part_stride, uint64_t part_stride_db)
+{
+    constexpr int WAVES = (TN / WN) * (TK / WK), WAVES_K = TK / WK, BT = 64, SLOTS = BT / 8, GROUPS = BT / 16;
+    constexpr int FN = WN / 32, FK = WK / 32, NT = 64 * WAVES;
+    constexpr int CX = TK / 4, XWAVES = SLOTS * CX / 64;                // waves with units (8 tokens x 4 columns) of x
+    constexpr int PIECES = TN / 32, LR = TN / 8, RP = 64 / LR;          // of a row of dy; lanes of a row, rows of a load
+    constexpr int ROWS = BT / WAVES, LOADS = ROWS / RP;                 // rows and loads of a wave
+    constexpr int TURN = PIECES < 4 ? PIECES - 1 : 3;
+    static_assert(XWAVES <= WAVES && LOADS * RP == ROWS, "units and waves");
+    __shared__ u32x4 left[2][BT * TN / 8];
+    __shared__ u32x4 right[2][TK * SLOTS];
+
+    uint32_t tr, tc;
+    tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, g = lane >> 5;
+    const int wn = (wave / WAVES_K) * WN, wk = (wave % WAVES_K) * WK;
+    const uint32_t stages = (t_rows + BT - 1) / BT;
+    const uint32_t first = blockIdx.y * stages_each, last = min(stages, first + stages_each);
+    const bool has_x = XWAVES == WAVES || wave < XWAVES;
+    const int x_slot0 = wave * 64 / CX, x_slot = x_slot0 + lane / CX, x_col = (lane % CX) * 4;
+    const uint32_t pitch = steps * kStep, pitch_s = steps * 4, col_x = tc * TK + x_col, ld2 = (uint32_t)lddy * 2;
+    const uint32_t safe = safe_tokens(t_rows, n, (tr + 1) * TN, lddy, pitch, (tc + 1) * TK);
+    const uint32_t at_x = (lane / CX) * 8 * pitch + x_col;
+    const uint32_t at_s = ((lane / CX) * 8 + (lane & 7)) * pitch_s + x_col / 32;
+
+    // Stages up to `safe` load whole tiles; the others element by element, with zeros past the ends.
+    const auto row_of = [&](int load) NKMX_INLINE { return wave * ROWS + load * RP + lane / LR; };
+    const auto fetch_d = [&](uint32_t stage, int buf) NKMX_INLINE {
+        const u32x4 from = buffer_of(dy + (uint64_t)(stage * BT) * lddy + tr * TN, (BT - 1) * ld2 + TN * 2);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int p = lane % LR, piece = (p >> 2) ^ (row_of(i) & TURN);
+            load_to_lds(from, row_of(i) * ld2 + piece * 64 + (p & 3) * 16, &left[buf][(wave * ROWS + i * RP) * LR]);
+        }
+    };
+    const auto copy_d = [&](uint32_t stage, int buf) NKMX_INLINE {
+        uint16_t* to = reinterpret_cast<uint16_t*>(left[buf]);
+#pragma unroll 1
+        for (int i = tid; i < BT * TN; i += NT) {
+            const int t = i / TN, c = i % TN;
+            uint16_t v = 0;
+            if (stage * BT + t < t_rows && tr * TN + c < n)
+                v = reinterpret_cast<const uint16_t*>(dy)[(uint64_t)(stage * BT + t) * lddy + tr * TN + c];
+            to[t * TN + ((c >> 5) ^ (t & TURN)) * 32 + (c & 31)] = v;
+        }
+    };
+    struct Unit {
+        uint32_t q[8], e;  // codes of 8 tokens x 4 columns; scale byte of token lane % 8 (see the kernel above)
+    };
+    const auto fetch_x = [&](Unit& u, uint32_t stage) NKMX_INLINE {
+        const uint32_t t = stage * BT + x_slot0 * 8;
+        const uint8_t* p = codes + (uint64_t)t * pitch + tc * TK;
+        u.e = (scales + (uint64_t)t * pitch_s + tc * (TK / 32))[at_s];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u.q[i] = *reinterpret_cast<const uint32_t*>(p + (uint64_t)i * pitch + at_x);
+    };
+    const auto copy_x = [&](Unit& u, uint32_t stage) NKMX_INLINE {
+        const uint32_t t = stage * BT + x_slot * 8;
+        const bool live = col_x < pitch;
+        u.e = 0;
+        if (live && t + (lane & 7) < t_rows) u.e = scales[(uint64_t)(t + (lane & 7)) * pitch_s + col_x / 32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            u.q[i] = 0u;
+            if (live && t + i < t_rows) u.q[i] = *reinterpret_cast<const uint32_t*>(codes + (uint64_t)(t + i) * pitch + col_x);
+        }
+    };
+    const auto put_x = [&](const Unit& u, const float (&scale)[8], int buf, int j) NKMX_INLINE {
+        const uint32_t c = x_col + j;
+        right[buf][c * SLOTS + (x_slot ^ swizzle_t<SLOTS>(c))] = eight_tokens(u.q, scale, j);
+    };
+
+    f32x16 acc[FN][FK] = {};
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* LdsShorts;
+    // Lane a of 16 reads 4 columns of token a / 4; lanes 0-31 take the first 8 tokens of an instruction's 16, and lanes
+    // 16-31 of each half the upper 16 of its 32 columns.
+    const int a16 = lane & 15;
+    const uint32_t at_l = ((lane >> 5) * 8 + (a16 >> 2)) * (TN * 2) + ((lane >> 4) & 1) * 32 + (a16 & 3) * 8;
+    const auto turned = [&](int buf, int t, int piece) NKMX_INLINE {  // 4 tokens from t of a column of the piece
+        const char* p = reinterpret_cast<const char*>(left[buf]) + at_l + ((piece ^ ((a16 >> 2) & TURN)) * 64) + t * (TN * 2);
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShorts)p);
+    };
+    const auto take_b = [&](bf16x8 (&b)[FK], int buf, int h) NKMX_INLINE {
+#pragma unroll
+        for (int j = 0; j < FK; ++j) {
+            const uint32_t c = wk + 32 * j + r;
+            b[j] = __builtin_bit_cast(bf16x8, right[buf][c * SLOTS + ((2 * h + g) ^ swizzle_t<SLOTS>(c))]);
+        }
+    };
+    const auto take_a = [&](bf16x8& a, int buf, int h, int i) NKMX_INLINE {
+        const s16x4 lo = turned(buf, 16 * h, wn / 32 + i), hi = turned(buf, 16 * h + 4, wn / 32 + i);
+        const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+        const u32x4 both = {l2[0], l2[1], h2[0], h2[1]};
+        a = __builtin_bit_cast(bf16x8, both);
+    };
+    // Sums of dy's columns, in the tiles of the first columns of x: a wave sums its tokens, a lane TN / 64 columns.
+    float sum_dy[TN / 64] = {};
+    const auto add_up = [&](int buf) NKMX_INLINE {
+        const bf16x2 ones = {(bf16)1.0f, (bf16)1.0f};
+#pragma unroll
+        for (int j = 0; j < TN / 64; ++j)
+#pragma unroll
+            for (int t = 0; t < ROWS; t += 4) {
+                const int piece = 2 * j + (lane >> 5);
+                const char* p = reinterpret_cast<const char*>(left[buf]) + (wave * ROWS + t + (a16 >> 2)) * (TN * 2) +
+                                ((piece ^ ((a16 >> 2) & TURN)) * 64) + ((lane >> 4) & 1) * 32 + (a16 & 3) * 8;
+                const u32x2 four = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShorts)p));
+                const uint32_t lo = four[0], hi = four[1];
+                sum_dy[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, lo), ones, sum_dy[j], false);
+                sum_dy[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, hi), ones, sum_dy[j], false);
+            }
+    };
+
+    bf16x8 a[FN], b[2][FK];
+    // The 16 tokens h of a stage.  An operand is read for the next 16 as soon as it has been used; the instructions of
+    // what `work` adds and the LDS reads go between the matrix instructions.
+    const auto tokens = [&](int buf, auto index, auto work) NKMX_INLINE {
+        constexpr int h = decltype(index)::value;
+        if constexpr (h + 1 < GROUPS) take_b(b[(h + 1) & 1], buf, h + 1);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+#pragma unroll
+            for (int j = 0; j < FK; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[h & 1][j], acc[i][j], 0, 0, 0);
+            if constexpr (h + 1 < GROUPS) take_a(a[i], buf, h + 1, i);
+        }
+        work();
+#pragma unroll
+        for (int z = 0; z < FN * FK; ++z) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // others
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // an LDS write
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    typedef std::integral_constant<int, 0> H0;
+    typedef std::integral_constant<int, 1> H1;
+    typedef std::integral_constant<int, 2> H2;
+    typedef std::integral_constant<int, 3> H3;
+    const auto run = [&](auto sums) NKMX_INLINE {
+        Unit now, next;
+        float scale[8];
+        // MORE: stages that follow and are loaded from this one, 2 (codes of the second, dy of the first), 1 or 0.
+        const auto stage = [&](uint32_t s, int buf, auto more) NKMX_INLINE {
+            constexpr int MORE = decltype(more)::value;
+            constexpr bool TURNS = MORE > 0 && XWAVES == WAVES;
+            take_b(b[0], buf, 0);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) take_a(a[i], buf, 0, i);
+            __builtin_amdgcn_sched_barrier(0);
+            tokens(buf, H0{}, [] {});
+            if constexpr (decltype(sums)::value) add_up(buf);
+            if constexpr (MORE > 0) {
+                if constexpr (XWAVES == WAVES) {
+                    // (as assembly, or the moves, and with them the wait for the loads, go to the stage's beginning)
+                    asm volatile("v_mov_b32 %0, %1" : "=v"(now.e) : "v"(next.e));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) asm volatile("v_mov_b32 %0, %1" : "=v"(now.q[i]) : "v"(next.q[i]));
+                    spread_scales(now.e, scale);
+                    fetch_d(s + 1, buf ^ 1);
+                    if constexpr (MORE > 1) fetch_x(next, s + 2);
+                } else {
+                    fetch_d(s + 1, buf ^ 1);
+                    if (has_x) {
+                        fetch_x(now, s + 1);
+                        spread_scales(now.e, scale);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) put_x(now, scale, buf ^ 1, j);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const auto turn = [&](int from, int to) NKMX_INLINE {
+                if constexpr (TURNS) {
+#pragma unroll
+                    for (int j = from; j < to; ++j) put_x(now, scale, buf ^ 1, j);
+                }
+            };
+            tokens(buf, H1{}, [&]() NKMX_INLINE { turn(0, 2); });
+            tokens(buf, H2{}, [&]() NKMX_INLINE { turn(0, 0); });
+            tokens(buf, H3{}, [&]() NKMX_INLINE { turn(2, 4); });
+            // dy has arrived when no more than the 9 loads of codes behind it are on their way (fewer, to be safe)
+            if constexpr (TURNS && MORE > 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else arrived();
+        };
+        const uint32_t fast = max(first, min(last, safe / BT));  // stages of whole tiles
+        if (first < fast) {
+            fetch_d(first, 0);
+            if (has_x) {
+                fetch_x(now, first);
+                spread_scales(now.e, scale);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) put_x(now, scale, 0, j);
+                if (XWAVES == WAVES && first + 1 < fast) fetch_x(next, first + 1);
+            }
+            arrived();
+            int buf = 0;
+            for (uint32_t s = first; s + 2 < fast; ++s, buf ^= 1) stage(s, buf, std::integral_constant<int, 2>{});
+            if (first + 1 < fast) {
+                stage(fast - 2, buf, std::integral_constant<int, 1>{});
+                buf ^= 1;
+            }
+            stage(fast - 1, buf, std::integral_constant<int, 0>{});
+        }
+#pragma unroll 1
+        for (uint32_t s = fast; s < last; ++s) {  // the last tokens
+            copy_d(s, 0);
+            if (has_x) {
+                copy_x(now, s);
+                spread_scales(now.e, scale);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) put_x(now, scale, 0, j);
+            }
+            arrived();
+            stage(s, 0, std::integral_constant<int, 0>{});
+        }
+    };
+    if (db != nullptr && tc == 0) run(std::true_type{});
+    else run(std::false_type{});
+
+    store_gradient<FN, FK>(acc, dw + blockIdx.y * part_stride, lddw, tr * TN + wn, tc * TK + wk, n, k, accumulate, r, g);
+    if (db != nullptr && tc == 0) {  // the waves' sums of a column, joined in order
+        float* part = reinterpret_cast<float*>(&right[0][0]);
+#pragma unroll
+        for (int j = 0; j < TN / 64; ++j) part[wave * TN + 64 * j + lane] = sum_dy[j];
+        __syncthreads();
+        for (int c = tid; c < TN; c += NT)
+            if (tr * TN + c < n) {
+                float s = part[c];
+#pragma unroll
+                for (int i = 1; i < WAVES; ++i) s += part[i * TN + c];
+                float* p = db + blockIdx.y * part_stride_db + tr * TN + c;
+                *p = accumulate ? *p + s : s;
+            }
     }
 }
 
@@ -1158,10 +1645,15 @@ inline int launch_wgrad(const WgradPlan& p, float* dw, uint64_t lddw, float* db,
 {
     const uint64_t tiles = p.row_tiles * p.col_tiles;
     if (tiles > kMaxSize || p.parts > 65535) return NKMX_ERANGE;
-    return launch(act8_wgrad_kernel<T, TN, TK, WN, WK, BT>, dim3((uint32_t)tiles, (uint32_t)p.parts),
-                  64 * (TN / WN) * (TK / WK), s, dw, lddw, db, dy, lddy, codes, scales, (uint32_t)t, (uint32_t)n,
-                  (uint32_t)k, (uint32_t)steps_of(k), (uint32_t)p.row_tiles, (uint32_t)p.col_tiles,
-                  (uint32_t)p.stages_each, accumulate, stride, stride);
+    const auto with = [&](auto kernel) {
+        return launch(kernel, dim3((uint32_t)tiles, (uint32_t)p.parts), 64 * (TN / WN) * (TK / WK), s, dw, lddw, db, dy, lddy,
+                      codes, scales, (uint32_t)t, (uint32_t)n, (uint32_t)k, (uint32_t)steps_of(k), (uint32_t)p.row_tiles,
+                      (uint32_t)p.col_tiles, (uint32_t)p.stages_each, accumulate, stride, stride);
+    };
+    if constexpr (std::is_same_v<T, bf16>) {
+        if (on(dy, 4) && lddy % 2 == 0 && lddy < (1u << 24)) return with(act8_wgrad_raw_kernel<TN, TK, WN, WK>);
+    }
+    return with(act8_wgrad_kernel<T, TN, TK, WN, WK, BT>);
 }
 
 }  // namespace
