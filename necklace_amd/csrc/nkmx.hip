@@ -490,11 +490,12 @@ __global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x
 
 // ---------------------------------------------------------------- mx4 product, few rows
 //
-// Few rows of a: the call reads b once and is bound by that.  A workgroup owns 16 rows of b and MT x 16 rows
-// of a; its 8 waves take the steps of k in turn, straight from memory into the operands of the matrix
-// instruction (16 x 16 x 128: lane l holds row l % 16 and block l / 16 of the step, 16 bytes as they are
-// stored), and their sums are joined through LDS in wave order.  FUSED: a lane quantizes its own block of
-// 32 numbers of x in registers, with the arithmetic of mx4_quantize_kernel.
+// Few rows of a: the call reads b once and is bound by that, and by the look-ups of its scattered lines.  A
+// workgroup owns 16 NT rows of b and 16 MT of a; its 8 waves take a run of the steps of k each, straight from memory
+// into the operands of the 16 x 16 x 128 instruction (lane l holds row l % 16 and block l / 16 of the step, 16 bytes as
+// they are stored: four lanes read 64 bytes of a row, and the next step's load the rest of the cache line), four
+// steps at a time with one load of their scales.  The waves' sums are joined through LDS in wave order.  FUSED: a lane
+// quantizes its own block of 32 numbers of x in registers, with the arithmetic of mx4_quantize_kernel.
 
 constexpr int kRowsWaves = 8;
 
@@ -503,78 +504,149 @@ __device__ __forceinline__ i32x8 operand4(u32x4 v)
     return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
 }
 
-// The block of 32 numbers that starts at p, `live` of them in the matrix, as an operand and its scale byte.
-template <typename T>
-__device__ __forceinline__ u32x4 quantize_block(const T* p, int64_t live, uint32_t& byte)
+// The waves' sums of a block of `rows` x `cols` (a power of two) results, in wave order, with the bias, into y.
+template <typename T, int SIZE>
+__device__ __forceinline__ void join_waves(const float (&sums)[kRowsWaves][SIZE], int cols, T* y, uint64_t ldy, const T* bias,
+                                           uint32_t m0, uint32_t n0, uint32_t m, uint32_t n)
 {
-    typedef typename Pack<T, 8>::vec V;
-    typedef typename Pack<T, 8>::loose L;
-    V v[4];
-    if (live >= 32) {
+    for (int i = threadIdx.x; i < SIZE; i += 64 * kRowsWaves) {
+        float s = sums[0][i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const L*>(p + 8 * i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i / 8][i % 8] = i < live ? p[i] : (T)0.0f;
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, magnitude(number(v[i / 8][i % 8])));
-    byte = scale_byte<2>(top);
-    const float scale = scale_value(byte);
-    u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = byte == 255u ? 0u : codes4<V, 8>(v[i], scale);
-    return w;
-}
-
-template <typename T, int MT, bool FUSED>
-__global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_t ldy, const T* x, uint64_t ldx,
-                                                                   const uint8_t* ca, const uint8_t* sa, const uint8_t* cb,
-                                                                   const uint8_t* sb, const T* bias, uint32_t m, uint32_t n,
-                                                                   uint32_t k, uint32_t steps)
-{
-    __shared__ float sums[kRowsWaves][MT][256];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
-    const uint64_t row_b = min(n0 + r, n - 1);
-    const u32x4* pb = reinterpret_cast<const u32x4*>(cb) + row_b * steps * 4 + g;
-    const uint32_t* qb = reinterpret_cast<const uint32_t*>(sb) + row_b * steps;
-    f32x4 acc[MT] = {};
-    for (uint32_t s = wave; s < steps; s += kRowsWaves) {
-        const i32x8 vb = operand4(pb[s * 4]);
-        const int eb = (int)((qb[s] >> (8 * g)) & 255u);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            u32x4 a = {0u, 0u, 0u, 0u};
-            uint32_t ea = 0;
-            if constexpr (FUSED) {
-                const uint32_t row = m0 + 16 * t + r;
-                const int64_t live = (int64_t)k - (int64_t)(s * kStep + g * 32);
-                if (row < m) a = quantize_block<T>(x + row * ldx + s * kStep + g * 32, live, ea);
-            } else {
-                const uint64_t row = min(m0 + 16 * t + r, m - 1);
-                a = reinterpret_cast<const u32x4*>(ca)[(row * steps + s) * 4 + g];
-                ea = (reinterpret_cast<const uint32_t*>(sa)[row * steps + s] >> (8 * g)) & 255u;
-            }
-            acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(a), vb, acc[t], 4, 4, 0, (int)ea, 0, eb);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[wave][t][(4 * g + i) * 16 + r] = acc[t][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += 64 * kRowsWaves) {
-        float s = sums[0][i >> 8][i & 255];
-#pragma unroll
-        for (int w = 1; w < kRowsWaves; ++w) s += sums[w][i >> 8][i & 255];
-        const uint32_t row = m0 + (i >> 4), col = n0 + (i & 15);
+        for (int w = 1; w < kRowsWaves; ++w) s += sums[w][i];
+        const uint32_t row = m0 + i / cols, col = n0 + i % cols;
         if (row < m && col < n) {
             if (bias) s += number(bias[col]);
             y[row * ldy + col] = (T)s;
         }
     }
+}
+
+template <typename V>
+__device__ __forceinline__ uint32_t eight_max(V v) { return lane_max(v); }
+__device__ __forceinline__ uint32_t eight_max(Pack<float, 8>::vec v)
+{
+    return max(lane_max(Pack<float, 4>::vec{v[0], v[1], v[2], v[3]}), lane_max(Pack<float, 4>::vec{v[4], v[5], v[6], v[7]}));
+}
+
+// A block of 32 numbers, `live` of them in the matrix, and its codes as an operand.
+template <typename T>
+struct Block {
+    typename Pack<T, 8>::vec v[4];
+    __device__ __forceinline__ void load(const T* p, int64_t live)
+    {
+        typedef typename Pack<T, 8>::loose L;
+        if (live >= 32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const L*>(p + 8 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i / 8][i % 8] = i < live ? p[i] : (T)0.0f;
+        }
+    }
+    __device__ __forceinline__ u32x4 codes(uint32_t& byte) const
+    {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, eight_max(v[i]));
+        byte = scale_byte<2>(top);
+        const float scale = scale_value(byte);
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t one = codes4<typename Pack<T, 8>::vec, 8>(v[i], scale);
+            w[i] = byte == 255u ? 0u : one;
+        }
+        return w;
+    }
+};
+
+template <typename T, int MT, int NT, bool FUSED>
+__global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_t ldy, const T* x, uint64_t ldx,
+                                                                   const uint8_t* ca, const uint8_t* sa, const uint8_t* cb,
+                                                                   const uint8_t* sb, const T* bias, uint32_t m, uint32_t n,
+                                                                   uint32_t k, uint32_t steps)
+{
+    __shared__ float sums[kRowsWaves][MT * NT * 256];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const uint32_t n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+    const u32x4 *pa[MT], *pb[NT];
+    const uint32_t *qa[MT], *qb[NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const uint64_t row = min(m0 + 16 * t + r, m - 1);
+        pa[t] = reinterpret_cast<const u32x4*>(ca) + row * steps * 4 + g;
+        qa[t] = reinterpret_cast<const uint32_t*>(sa) + row * steps;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const uint64_t row = min(n0 + 16 * t + r, n - 1);
+        pb[t] = reinterpret_cast<const u32x4*>(cb) + row * steps * 4 + g;
+        qb[t] = reinterpret_cast<const uint32_t*>(sb) + row * steps;
+    }
+    f32x4 acc[MT][NT] = {};
+    typedef u32x4 Loose __attribute__((aligned(4)));
+    const auto some = [&](uint32_t s, auto count) NKMX_INLINE {
+        constexpr int N = decltype(count)::value;
+        u32x4 a[N][MT], b[N][NT], ea[MT], eb[NT];
+        const auto scales = [&](const uint32_t* q) NKMX_INLINE {
+            if constexpr (N == 4) return *reinterpret_cast<const Loose*>(q + s);
+            else return u32x4{q[s], 0u, 0u, 0u};
+        };
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            eb[t] = scales(qb[t]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) b[i][t] = pb[t][(s + i) * 4];
+        }
+        Block<T> raw[FUSED ? N : 1][FUSED ? MT : 1];
+        if constexpr (FUSED) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const uint32_t row = m0 + 16 * t + r, col = (s + i) * kStep + g * 32;
+                    if (row < m) raw[i][t].load(x + row * ldx + col, (int64_t)k - (int64_t)col);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                ea[t] = scales(qa[t]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) a[i][t] = pa[t][(s + i) * 4];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                uint32_t e;
+                if constexpr (FUSED) {
+                    a[i][t] = raw[i][t].codes(e);
+                    if (m0 + 16 * t + r >= m) {
+                        a[i][t] = u32x4{0u, 0u, 0u, 0u};
+                        e = 0;
+                    }
+                } else {
+                    e = (ea[t][i] >> (8 * g)) & 255u;
+                }
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+                    acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        operand4(a[i][t]), operand4(b[i][u]), acc[t][u], 4, 4, 0, (int)e, 0, (int)((eb[u][i] >> (8 * g)) & 255u));
+            }
+    };
+    const uint32_t each = (steps + kRowsWaves - 1) / kRowsWaves, end = min(steps, (wave + 1) * each);
+    uint32_t s = wave * each;
+    for (; s + 4 <= end; s += 4) some(s, std::integral_constant<int, 4>{});
+    for (; s < end; ++s) some(s, std::integral_constant<int, 1>{});
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[wave][(16 * t + 4 * g + i) * (16 * NT) + 16 * u + r] = acc[t][u][i];
+    __syncthreads();
+    join_waves(sums, 16 * NT, y, ldy, bias, m0, n0, m, n);
 }
 
 // ---------------------------------------------------------------- tiles
@@ -624,13 +696,15 @@ __device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t at, const voi
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(base), "v"(at), "s"(buffer) : "memory");
 }
-// This wave's loads to LDS have arrived, and everybody's; what was read before is free to be overwritten.
+// All but the latest LATER loads of every wave have arrived in LDS; what the waves read before is free to be
+// overwritten.
+template <int LATER = 0>
 __device__ __forceinline__ void arrived()
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LATER) : "memory");
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, int TM, int TN, int WM, int WN, int BUFFERS>
 __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
     T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb, const T* bias,
     uint32_t m, uint32_t n, uint32_t steps, uint32_t row_tiles, uint32_t col_tiles)
@@ -638,8 +712,8 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
     constexpr int WAVES = (TM / WM) * (TN / WN), WAVES_N = TN / WN;
     constexpr int FM = WM / 32, FN = WN / 32;
     static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && WAVES % 2 == 0, "whole rounds of row groups");
-    __shared__ u32x4 image[2][(TM + TN) * 8];
-    __shared__ uint32_t bytes[2][(TM + TN) * kSpan];
+    __shared__ u32x4 image[BUFFERS][(TM + TN) * 8];
+    __shared__ uint32_t bytes[BUFFERS][(TM + (TN < 64 ? 64 : TN)) * kSpan];  // loads of scales are 64 rows long
 
     uint32_t tr, tc;
     tile_of(blockIdx.x, row_tiles, col_tiles, tr, tc);
@@ -657,7 +731,8 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
     const uint32_t at = (lane >> 3) * pitch + (((lane & 7) ^ swizzle8((wave & 1) * 8 + (lane >> 3))) << 4);
     const uint32_t at_s = lane * pitch_s;  // 64 rows a load
 
-    const auto fetch = [&](uint32_t stage, int buf) {
+    const auto fetch = [&](uint32_t stage) {
+        const int buf = stage % BUFFERS;
 #pragma unroll
         for (int i = 0; i < TM / 8 / WAVES; ++i) {
             const int group = i * WAVES + wave;
@@ -672,12 +747,12 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
         // load costs
         if ((stage & 1) == 0) {
 #pragma unroll
-            for (int i = 0; i < ((TM + TN) / 64 + WAVES - 1) / WAVES; ++i) {
+            for (int i = 0; i < (TM / 64 + (TN + 63) / 64 + WAVES - 1) / WAVES; ++i) {
                 const int group = i * WAVES + wave;
-                uint32_t* to = &bytes[(stage >> 1) & 1][group * 64 * kSpan];
+                uint32_t* to = &bytes[(stage >> 1) % BUFFERS][group * 64 * kSpan];
                 if (group < TM / 64)
                     load_to_lds(buf_sa, at_s + (group * 64 * pitch_s + stage * 8), to);
-                else if (group < (TM + TN) / 64)
+                else if (group < TM / 64 + (TN + 63) / 64)
                     load_to_lds(buf_sb, at_s + ((group - TM / 64) * 64 * pitch_s + stage * 8), to);
             }
         }
@@ -701,7 +776,7 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
         int a[FM], b[FN];
     };
     const auto take_scales = [&](Scales& e, uint32_t stage) {
-        const uint32_t* from = bytes[(stage >> 1) & 1] + (stage & 1) * 2 + g;
+        const uint32_t* from = bytes[(stage >> 1) % BUFFERS] + (stage & 1) * 2 + g;
 #pragma unroll
         for (int i = 0; i < FM; ++i) e.a[i] = from[(wm + 32 * i + r) * kSpan];
 #pragma unroll
@@ -733,10 +808,28 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
 
     Operands o, p;
     Scales e, f;
-    const auto one_stage = [&](uint32_t s, const Scales& now, Scales& next) {
-        const int buf = s & 1;
-        if (s + 1 < stages) fetch(s + 1, buf ^ 1);
+    // Loads of a stage that every wave issues at least; so many of each later stage may be on their way.
+    constexpr int LOADS = (TM + TN) / 8 / WAVES;
+    const auto one_stage = [&](uint32_t s, const Scales& now, Scales& next, auto more) {
+        const int buf = s % BUFFERS;
+        if constexpr (decltype(more)::value) fetch(s + BUFFERS - 1);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (FM * FN == 1) {  // one instruction each: what counts is the chain of waits, so everything is read at once
+            Operands v, w;
+            take(p, buf, 1);
+            take(v, buf, 2);
+            take(w, buf, 3);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(o, now, std::integral_constant<int, 0>{});
+            multiply(p, now, std::integral_constant<int, 1>{});
+            arrived<decltype(more)::value ? (BUFFERS - 2) * LOADS : 0>();
+            take(o, (s + 1) % BUFFERS, 0);
+            take_scales(next, s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(v, now, std::integral_constant<int, 2>{});
+            multiply(w, now, std::integral_constant<int, 3>{});
+            return;
+        }
         take(p, buf, 1);
         multiply(o, now, std::integral_constant<int, 0>{});
         interleave(One{});
@@ -748,24 +841,29 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
         interleave(One{});
         // this stage has been read; what follows reads the next one while the last instructions run (after the last
         // stage: what is there, unused)
-        arrived();
-        take(o, buf ^ 1, 0);
+        arrived<decltype(more)::value ? (BUFFERS - 2) * LOADS : 0>();
+        take(o, (s + 1) % BUFFERS, 0);
         take_scales(next, s + 1);
         multiply(p, now, std::integral_constant<int, 3>{});
         interleave(Two{});
     };
     const uint32_t whole = steps / 2;
-    fetch(0, 0);
+    for (uint32_t s = 0; s + 1 < BUFFERS && s < stages; ++s) fetch(s);
     arrived();
     take(o, 0, 0);
     take_scales(e, 0);
-    for (uint32_t s = 0; s < whole; ++s) {
-        one_stage(s, e, f);
+    uint32_t s = 0;
+    for (; s + BUFFERS - 1 < stages; ++s) {
+        one_stage(s, e, f, std::true_type{});
+        e = f;
+    }
+    for (; s < whole; ++s) {
+        one_stage(s, e, f, std::false_type{});
         e = f;
     }
     if (steps & 1) {  // half a stage: the lanes of its second step take part with zeros
         const auto rest = [&](auto index) {
-            if (decltype(index)::value) take(o, whole & 1, decltype(index)::value);
+            if (decltype(index)::value) take(o, whole % BUFFERS, decltype(index)::value);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 if (g) o.a[i] = u32x4{0u, 0u, 0u, 0u};
@@ -1571,42 +1669,56 @@ inline Area scale_bytes(const void* p, uint64_t rows, uint64_t cols) { return ru
 
 // ---- product
 
-constexpr uint64_t kRowsMax = 64;       // rows of a that the few-rows kernel takes
-constexpr uint64_t kFusedRowsMax = 8;   // rows of x that are quantized inside the product
+// A tile's rows lie within the 4 GB that a buffer load can address: 256 rows of k / 2 bytes.
+constexpr uint64_t kTilesMaxK = 1ull << 24;
+// Whether x is quantized inside the product: every workgroup (16 rows of b) then quantizes all of x, 100 instructions a
+// step of k and wave, which a launch saved pays for while b is small (us, inside / before, captured): 1 x 4096 x 1024 3.0 /
+// 4.3, 8 x 1024 x 4096 5.9 / 5.8, 1 x 8192 x 8192 12.6 / 10.4.  A call made eagerly saves 4 us of host time as well.
+inline bool quantizes_inside(uint64_t m, uint64_t n, uint64_t k) { return m <= 8 && k && n * k <= 1ull << 24; }
 
-template <typename T, int MT, bool FUSED>
+template <typename T, int MT, int NT, bool FUSED>
 inline int launch_rows(T* y, uint64_t ldy, const T* x, uint64_t ldx, const uint8_t* ca, const uint8_t* sa,
                        const uint8_t* cb, const uint8_t* sb, const T* bias, uint64_t m, uint64_t n, uint64_t k,
                        hipStream_t s)
 {
-    const dim3 grid((uint32_t)((n + 15) / 16), (uint32_t)((m + 16 * MT - 1) / (16 * MT)));
-    return launch(mx4_rows_kernel<T, MT, FUSED>, grid, 64 * kRowsWaves, s, y, ldy, x, ldx, ca, sa, cb, sb, bias,
+    const dim3 grid((uint32_t)((n + 16 * NT - 1) / (16 * NT)), (uint32_t)((m + 16 * MT - 1) / (16 * MT)));
+    return launch(mx4_rows_kernel<T, MT, NT, FUSED>, grid, 64 * kRowsWaves, s, y, ldy, x, ldx, ca, sa, cb, sb, bias,
                   (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)steps_of(k));
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, int TM, int TN, int WM, int WN, int BUFFERS>
 inline int launch_tiles(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb,
                         const T* bias, uint64_t m, uint64_t n, uint64_t k, hipStream_t s)
 {
     const uint64_t rt = (m + TM - 1) / TM, ct = (n + TN - 1) / TN;
     if (rt * ct > kMaxSize) return NKMX_ERANGE;
-    return launch(mx4_tiles_kernel<T, TM, TN, WM, WN>, dim3((uint32_t)(rt * ct)), 64 * (TM / WM) * (TN / WN), s, y, ldy,
+    return launch(mx4_tiles_kernel<T, TM, TN, WM, WN, BUFFERS>, dim3((uint32_t)(rt * ct)), 64 * (TM / WM) * (TN / WN), s, y, ldy,
                   ca, sa, cb, sb, bias, (uint32_t)m, (uint32_t)n, (uint32_t)steps_of(k), (uint32_t)rt, (uint32_t)ct);
 }
 
+// Which kernel, by counts of workgroups (us at m x n x k, codes from HBM):
+//   rows 16 x 16      up to 16 rows, and while there are at most 384 of them: 64 x 1024 x 4096 4.8 against 8.0 by tiles,
+//                     100 x 1024 x 1024 (448) 4.2 against 4.4, 200 x 1024 x 1024 (832) 6.6 against 4.4
+//   rows 32 x 32      up to 32 rows: 32 x 8192 x 8192 15.1 against 15.3 by tiles of 64, and 22.7 by rows of 16
+//   tiles 256         from 192 tiles: 4096^3 43 against 55 by tiles of 128; 2048 x 4096 x 4096 (128 tiles) 33 against 26
+//   tiles 128         from 192 tiles: 1024 x 4096 x 4096 17 against 22 by tiles of 64; 512 x 4096 x 4096 (128) 15 against
+//                     12.6; with four buffers while every workgroup has a CU of its own (512 x 8192 x 8192 30 against 41
+//                     with two), with two beyond (2048 x 4096 x 4096 26.6 against 30.3)
+//   tiles 64 x 32     up to 128 tiles of 64: 64 x 8192 x 8192 15.0 against 17.2, but 128 x 8192 x 8192 21 against 17
 template <typename T>
 int product(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb,
             const T* bias, uint64_t m, uint64_t n, uint64_t k, hipStream_t s)
 {
-    if (k == 0 || m <= kRowsMax) {
-        if (m <= 16) return launch_rows<T, 1, false>(y, ldy, nullptr, 0, ca, sa, cb, sb, bias, m, n, k, s);
-        if (m <= 32) return launch_rows<T, 2, false>(y, ldy, nullptr, 0, ca, sa, cb, sb, bias, m, n, k, s);
-        return launch_rows<T, 4, false>(y, ldy, nullptr, 0, ca, sa, cb, sb, bias, m, n, k, s);
-    }
     const auto tiles = [&](uint64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
-    if (tiles(256) >= 192) return launch_tiles<T, 256, 256, 128, 64>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
-    if (tiles(128) >= 192) return launch_tiles<T, 128, 128, 64, 64>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
-    return launch_tiles<T, 64, 64, 32, 32>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    const T* none = nullptr;
+    if (m <= 16 || tiles(16) <= 384) return launch_rows<T, 1, 1, false>(y, ldy, none, 0, ca, sa, cb, sb, bias, m, n, k, s);
+    if (k == 0 || m <= 32 || k > kTilesMaxK)
+        return launch_rows<T, 2, 2, false>(y, ldy, none, 0, ca, sa, cb, sb, bias, m, n, k, s);
+    if (tiles(256) >= 192) return launch_tiles<T, 256, 256, 128, 64, 2>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    if (tiles(128) > 256) return launch_tiles<T, 128, 128, 64, 64, 2>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    if (tiles(128) >= 192) return launch_tiles<T, 128, 128, 64, 64, 4>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    if (tiles(64) > 128) return launch_tiles<T, 64, 64, 32, 32, 4>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
+    return launch_tiles<T, 64, 32, 32, 32, 4>(y, ldy, ca, sa, cb, sb, bias, m, n, k, s);
 }
 
 // ---- weight gradient
@@ -1745,7 +1857,7 @@ int nkmx_mx4_matmul(void* y, int type, uint64_t m, uint64_t n, uint64_t k, uint6
 
 uint64_t nkmx_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k)
 {
-    if (m <= kFusedRowsMax || m > kMaxSize || n == 0 || n > kMaxSize || k > kMaxSize) return 0;
+    if (m > kMaxSize || n == 0 || n > kMaxSize || k > kMaxSize || quantizes_inside(m, n, k)) return 0;
     return m * steps_of(k) * (kStepBytes4 + 4);
 }
 
@@ -1772,8 +1884,8 @@ int nkmx_mx4_linear(void* y, const void* x, int type, uint64_t m, uint64_t n, ui
     if (need) NKMX_TRY(nkmx_mx4_quantize(x, type, m, k, ldx, ca, sa, 0, stream));
     return for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
-        if (m <= kFusedRowsMax && k)
-            return launch_rows<T, 1, true>((T*)y, ldy, (const T*)x, ldx, nullptr, nullptr, b_codes, b_scales,
+        if (quantizes_inside(m, n, k))
+            return launch_rows<T, 1, 1, true>((T*)y, ldy, (const T*)x, ldx, nullptr, nullptr, b_codes, b_scales,
                                            (const T*)bias, m, n, k, s);
         return product<T>((T*)y, ldy, ca, sa, b_codes, b_scales, (const T*)bias, m, n, k, s);
     });

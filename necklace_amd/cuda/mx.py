@@ -19,11 +19,13 @@ Tensors of numbers are float32, bfloat16 or float16 and may be column ranges of 
 dimension, columns next to each other); more than two dimensions are taken as rows of the last one where that needs
 no copy, one dimension as a single row.  Outputs may not overlap inputs unless a call says so.
 """
+import functools
+
 import torch
 
 from .. import _lib
 from . import nbutils
-from .quantize import _finish, _on_device
+from .quantize import _finish
 
 BLOCK = 32
 STEP = 128
@@ -86,6 +88,18 @@ def row_stride(t):
 
 
 def _matrix(name, t):
+    """(rows, columns, leading dimension) of a tensor of numbers."""
+    try:
+        if t.dim() == 2 and t.is_cuda and t.dtype in _TYPES:  # what nearly every call brings
+            rows, cols = t.shape
+            ld, one = t.stride()
+            if one == 1:
+                if rows == 1:
+                    return 1, cols, cols
+                if ld >= cols and rows > 1:
+                    return rows, cols, ld
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
     if t.dtype not in _TYPES:
@@ -108,9 +122,15 @@ def _same_type(name, t, other, want):
 
 def _packed(name, c, s, rows, cols, mx4, what):
     """Checks codes `c` and scales `s` against the matrix they stand for."""
-    steps = steps_of(cols)
-    for part, t, dtype, width in ((name, c, torch.uint8 if mx4 else torch.int8, steps * (64 if mx4 else STEP)),
-                                  (f"scales of {name}", s, torch.uint8, steps * 4)):
+    steps = (cols + STEP - 1) // STEP
+    width, dtype = (steps * 64, torch.uint8) if mx4 else (steps * STEP, torch.int8)
+    try:
+        if c.shape == (rows, width) and s.shape == (rows, steps * 4) and c.dtype is dtype and s.dtype is torch.uint8 \
+                and c.is_cuda and s.is_cuda and c.is_contiguous() and s.is_contiguous():
+            return
+    except AttributeError:
+        pass
+    for part, t, dtype, width in ((name, c, dtype, width), (f"scales of {name}", s, torch.uint8, steps * 4)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{part}: expected a torch tensor, got {type(t).__name__}")
         if t.dtype != dtype:
@@ -123,29 +143,57 @@ def _packed(name, c, s, rows, cols, mx4, what):
             raise ValueError(f"{part}: must be contiguous")
 
 
-def _device(*tensors):
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t is not None and t.device != dev:
+def _device(first, *others):
+    """Index of the GPU that all tensors are on."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
             raise ValueError("all tensors must be on the same GPU")
     return dev
+
+
+class _on_device:
+    """`with torch.cuda.device(index)` only when that is not the current one already."""
+    __slots__ = ("ctx",)
+
+    def __init__(self, index):
+        self.ctx = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            return self.ctx.__exit__(*exc)
+        return False
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(m, n, k):
+    return int(_lib.mx_lib().nkmx_mx4_linear_workspace(m, n, k))
+
+
+@functools.lru_cache(maxsize=4096)
+def _wgrad_bytes(ty, t, n, k):
+    return int(_lib.mx_lib().nkmx_act8_wgrad_workspace(ty, t, n, k))
 
 
 def _workspace(given, need, dev, stream, handle):
     """`given`, or fresh memory of the stream that the call runs on."""
     if given is not None:
         if not isinstance(given, torch.Tensor) or given.dtype != torch.uint8 or not given.is_contiguous() \
-                or given.device != dev:
+                or given.get_device() != dev:
             raise TypeError("workspace: expected a contiguous uint8 tensor on the same GPU")
         return given
     if not need:
         return None
     if stream is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev)
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(handle, device=dev) if handle else torch.cuda.default_stream(dev)
+        stream = torch.cuda.ExternalStream(handle, device=torch.device("cuda", dev)) if handle else torch.cuda.default_stream(dev)
     with torch.cuda.stream(stream):  # the allocator hands a block on within its own stream only
-        return torch.empty(need, dtype=torch.uint8, device=dev)
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
 
 
 def _bias(bias, n, y):
@@ -212,7 +260,7 @@ def cu_fn_mx4_matmul_e(Y, CA, SA, CB, SB, bias=None, stream=None, sync=True):
 
 def mx4_linear_workspace(m, n, k):
     """Bytes of workspace that `cu_fn_mx4_linear_e` needs."""
-    return int(_lib.mx_lib().nkmx_mx4_linear_workspace(m, n, k))
+    return _linear_bytes(m, n, k)
 
 
 def cu_fn_mx4_linear_e(Y, X, CB, SB, bias=None, workspace=None, stream=None, sync=True):
@@ -232,7 +280,7 @@ def cu_fn_mx4_linear_e(Y, X, CB, SB, bias=None, workspace=None, stream=None, syn
     L = _lib.mx_lib()
     with _on_device(dev):
         h = nbutils.stream_handle(stream, dev)
-        ws = _workspace(workspace, L.nkmx_mx4_linear_workspace(m, n, k), dev, stream, h)
+        ws = _workspace(workspace, _linear_bytes(m, n, k), dev, stream, h)
         code = L.nkmx_mx4_linear(Y.data_ptr(), X.data_ptr(), _TYPES[Y.dtype], m, n, k, ldy, ldx, CB.data_ptr(),
                                  SB.data_ptr(), b, ws.data_ptr() if ws is not None else None,
                                  ws.numel() if ws is not None else 0, h)
@@ -308,7 +356,7 @@ def cu_fn_act8_grad_e(DX, DY, C, S, fn, stream=None, sync=True):
 
 def act8_wgrad_workspace(dtype, t, n, k):
     """Bytes of workspace that `cu_fn_act8_wgrad_e` needs for gradients DY of `dtype`."""
-    return int(_lib.mx_lib().nkmx_act8_wgrad_workspace(_TYPES[dtype], t, n, k))
+    return _wgrad_bytes(_TYPES[dtype], t, n, k)
 
 
 def cu_fn_act8_wgrad_e(DW, DY, C, S, DB=None, accumulate=False, workspace=None, stream=None, sync=True):
@@ -335,7 +383,7 @@ def cu_fn_act8_wgrad_e(DW, DY, C, S, DB=None, accumulate=False, workspace=None, 
     ty = _TYPES[DY.dtype]
     with _on_device(dev):
         h = nbutils.stream_handle(stream, dev)
-        ws = _workspace(workspace, L.nkmx_act8_wgrad_workspace(ty, t, n, k), dev, stream, h)
+        ws = _workspace(workspace, _wgrad_bytes(ty, t, n, k), dev, stream, h)
         code = L.nkmx_act8_wgrad(DW.data_ptr(), db, DY.data_ptr(), ty, t, n, k, lddw, lddy, C.data_ptr(), S.data_ptr(),
                                  1 if accumulate else 0, ws.data_ptr() if ws is not None else None,
                                  ws.numel() if ws is not None else 0, h)
