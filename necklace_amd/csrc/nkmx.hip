@@ -78,19 +78,19 @@ __device__ __forceinline__ float scale_value(uint32_t byte)
 // 2^(127 - byte) for bytes up to 253 (a finite number's byte is 252 at most).
 __device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// Phi(x) = erfc(-x / sqrt 2) / 2 with Abramowitz and Stegun's formula 7.1.26, erfc(z) = (a1 t + .. + a5 t^5)
-// e^(-z^2), t = 1 / (1 + p z) for z >= 0, |error| <= 1.5e-7; `tail` gets e^(-x^2 / 2).
-__device__ __forceinline__ float normal_distribution(float x, float& tail)
+// erfc(|x| / sqrt 2) / 2, the normal distribution's smaller side, by Abramowitz and Stegun's formula 7.1.26: erfc(z) =
+// (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), |error| <= 1.5e-7 (the factors 1 / sqrt 2 and 1 / 2 are in the
+// constants).  `tail` gets e^(-x^2 / 2).
+__device__ __forceinline__ float smaller_side(float x, float& tail)
 {
-    const float z = fabsf(x) * 0.70710678118654752f;
-    tail = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.0f));
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    const float half = 0.5f * (p * t * tail);
-    return x < 0.0f ? half : 1.0f - half;
+    const float u = x * 0.84932180028801905f;  // u^2 = x^2 / (2 ln 2)
+    tail = __builtin_amdgcn_exp2f(-(u * u));
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.3275911f * 0.70710678118654752f, 1.0f));
+    float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = fmaf(p, t, 0.5f * 1.421413741f);
+    p = fmaf(p, t, 0.5f * -0.284496736f);
+    p = fmaf(p, t, 0.5f * 0.254829592f);
+    return p * t * tail;
 }
 
 __device__ __forceinline__ float logistic(float x)
@@ -98,16 +98,25 @@ __device__ __forceinline__ float logistic(float x)
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
+// fn(x) of a number.
 template <int FN>
 __device__ __forceinline__ float activation(float x)
 {
-    if constexpr (FN == NKMX_GELU) {
+    if constexpr (FN == NKMX_GELU) {  // x Phi(x), without a choice by x's sign
         float tail;
-        return x * normal_distribution(x, tail);
+        return fmaf(-fabsf(x), smaller_side(x, tail), fmaxf(x, 0.0f));
     } else if constexpr (FN == NKMX_SILU) {
         return x * logistic(x);
     }
     return x;
+}
+// The same where x may be infinite or NaN: infinity stays, minus infinity times 0 is a NaN.
+template <int FN>
+__device__ __forceinline__ float activation_of_any(float x)
+{
+    const float y = activation<FN>(x);
+    if (FN == NKMX_GELU && magnitude(x) >= kInfBits) return x > 0.0f ? x : __uint_as_float(0x7FC00000u);
+    return y;
 }
 
 template <int FN>
@@ -115,8 +124,8 @@ __device__ __forceinline__ float activation_slope(float x)
 {
     if constexpr (FN == NKMX_GELU) {
         float tail;
-        const float phi = normal_distribution(x, tail);
-        return fmaf(x * 0.39894228040143268f, tail, phi);
+        const float side = smaller_side(x, tail);
+        return fmaf(x * 0.39894228040143268f, tail, x < 0.0f ? side : 1.0f - side);
     } else if constexpr (FN == NKMX_SILU) {
         const float s = logistic(x);
         return s * fmaf(x, 1.0f - s, 1.0f);
@@ -221,12 +230,13 @@ struct Place {
     int64_t live;      // elements of the matrix from this one on, to the end of the row (<= 0 in the padding)
 };
 
-template <typename T>
-__device__ __forceinline__ bool place_of(Place& p, FastDiv steps, uint32_t n_steps, uint32_t cols)
+// The lane's place number u of U: a wave takes U x 64 neighbouring ones.
+template <typename T, int U>
+__device__ __forceinline__ bool place_of(Place& p, int u, FastDiv steps, uint32_t n_steps, uint32_t cols)
 {
-    p.lane = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    p.lane = (uint64_t)blockIdx.x * (256 * U) + (threadIdx.x >> 6) * (64 * U) + u * 64 + (threadIdx.x & 63);
     const uint64_t step = p.lane / Lanes<T>::step;
-    if (step >= n_steps) return false;  // all lanes of a step leave together
+    if (step >= n_steps) return false;  // all lanes of a step together
     p.row = quotient((uint32_t)step, steps);
     p.col = ((uint32_t)step - p.row * steps.d) * kStep + (uint32_t)(p.lane % Lanes<T>::step) * Lanes<T>::E;
     p.live = (int64_t)cols - (int64_t)p.col;
@@ -299,20 +309,29 @@ __device__ __forceinline__ uint32_t codes4(V v, float scale)  // N = 4 or 8 valu
     return w;
 }
 
-template <typename T>
+template <typename T, int U>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* x, uint64_t ldx, uint8_t* codes, uint8_t* scales,
                                                            FastDiv steps, uint32_t n_steps, uint32_t cols)
 {
     constexpr int E = Lanes<T>::E;
-    Place p;
-    if (!place_of<T>(p, steps, n_steps, cols)) return;
-    const auto v = load_pack<T, E>(x + p.row * ldx + p.col, p.live);
-    const uint32_t byte = scale_byte<2>(block_max<Lanes<T>::block>(lane_max(v)));
-    uint32_t w = codes4<decltype(v), E>(v, scale_value(byte));
-    if (byte == 255u) w = 0u;
-    typedef typename Word<E / 2>::type W;
-    reinterpret_cast<W*>(codes)[p.lane] = (W)w;
-    store_scales<T>(scales, p, byte);
+    Place p[U];
+    bool in[U];
+    typename Pack<T, E>::vec v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        in[u] = place_of<T, U>(p[u], u, steps, n_steps, cols);
+        if (in[u]) v[u] = load_pack<T, E>(x + p[u].row * ldx + p[u].col, p[u].live);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (!in[u]) break;
+        const uint32_t byte = scale_byte<2>(block_max<Lanes<T>::block>(lane_max(v[u])));
+        uint32_t w = codes4<typename Pack<T, E>::vec, E>(v[u], scale_value(byte));
+        if (byte == 255u) w = 0u;
+        typedef typename Word<E / 2>::type W;
+        reinterpret_cast<W*>(codes)[p[u].lane] = (W)w;
+        store_scales<T>(scales, p[u], byte);
+    }
 }
 
 // q = x / 2^e to the nearest whole number: adding 1.5 * 2^23 in one rounding leaves it in the low bits, so
@@ -331,36 +350,49 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
     return ab | cd;
 }
 
-template <typename T, int FN>
+template <typename T, int FN, int U>
 __global__ __launch_bounds__(256) void act8_save_kernel(const T* x, uint64_t ldx, T* y, uint64_t ldy, uint8_t* codes,
                                                         uint8_t* scales, FastDiv steps, uint32_t n_steps, uint32_t cols)
 {
     constexpr int E = Lanes<T>::E;
-    Place p;
-    if (!place_of<T>(p, steps, n_steps, cols)) return;
-    const auto v = load_pack<T, E>(x + p.row * ldx + p.col, p.live);
-    const uint32_t byte = scale_byte<6>(block_max<Lanes<T>::block>(lane_max(v)));
-    const float inverse = scale_inverse(byte == 255u ? 0u : byte);
-    uint32_t q[E];
+    Place p[U];
+    bool in[U];
+    typename Pack<T, E>::vec v[U];
 #pragma unroll
-    for (int i = 0; i < E; ++i) q[i] = whole8(number(v[i]), inverse);
-    typedef typename Word<E>::type W;
-    W w;
-    if constexpr (E == 8) {
-        w[0] = low_bytes(q[0], q[1], q[2], q[3]);
-        w[1] = low_bytes(q[4], q[5], q[6], q[7]);
-        if (byte == 255u) w = W{0u, 0u};
-    } else {
-        w = low_bytes(q[0], q[1], q[2], q[3]);
-        if (byte == 255u) w = 0u;
+    for (int u = 0; u < U; ++u) {
+        in[u] = place_of<T, U>(p[u], u, steps, n_steps, cols);
+        if (in[u]) v[u] = load_pack<T, E>(x + p[u].row * ldx + p[u].col, p[u].live);
     }
-    reinterpret_cast<W*>(codes)[p.lane] = w;
-    store_scales<T>(scales, p, byte);
-    if constexpr (FN != NKMX_NONE) {
-        typename Pack<T, E>::vec o;
 #pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = (T)activation<FN>(number(v[i]));
-        store_pack<T, E>(y + p.row * ldy + p.col, o, p.live);
+    for (int u = 0; u < U; ++u) {
+        if (!in[u]) break;
+        const uint32_t byte = scale_byte<6>(block_max<Lanes<T>::block>(lane_max(v[u])));
+        const float inverse = scale_inverse(byte == 255u ? 0u : byte);
+        uint32_t q[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) q[i] = whole8(number(v[u][i]), inverse);
+        typedef typename Word<E>::type W;
+        W w;
+        if constexpr (E == 8) {
+            w[0] = low_bytes(q[0], q[1], q[2], q[3]);
+            w[1] = low_bytes(q[4], q[5], q[6], q[7]);
+            if (byte == 255u) w = W{0u, 0u};
+        } else {
+            w = low_bytes(q[0], q[1], q[2], q[3]);
+            if (byte == 255u) w = 0u;
+        }
+        reinterpret_cast<W*>(codes)[p[u].lane] = w;
+        store_scales<T>(scales, p[u], byte);
+        if constexpr (FN != NKMX_NONE) {
+            typename Pack<T, E>::vec o;
+#pragma unroll
+            for (int i = 0; i < E; ++i) o[i] = (T)activation<FN>(number(v[u][i]));
+            if (byte == 255u) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) o[i] = (T)activation_of_any<FN>(number(v[u][i]));
+            }
+            store_pack<T, E>(y + p[u].row * ldy + p[u].col, o, p[u].live);
+        }
     }
 }
 
@@ -372,72 +404,100 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float& a, float
     b = v[1];
 }
 
-template <typename T>
+template <typename T, int U>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(T* out, uint64_t ldo, const uint8_t* codes,
                                                              const uint8_t* scales, FastDiv steps, uint32_t n_steps,
                                                              uint32_t cols)
 {
     constexpr int E = Lanes<T>::E;
-    Place p;
-    if (!place_of<T>(p, steps, n_steps, cols)) return;
     typedef typename Word<E / 2>::type W;
-    const uint32_t w = reinterpret_cast<const W*>(codes)[p.lane];
-    const uint32_t byte = scales[p.lane / Lanes<T>::block];
-    const float scale = scale_value(byte == 255u ? 127u : byte);
-    float f[8];
-    values4<0>(w, scale, f[0], f[1]);
-    values4<1>(w, scale, f[2], f[3]);
-    if constexpr (E == 8) {
-        values4<2>(w, scale, f[4], f[5]);
-        values4<3>(w, scale, f[6], f[7]);
-    }
-    typename Pack<T, E>::vec o;
+    Place p[U];
+    bool in[U];
+    W code[U];
+    uint8_t e[U];
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = (T)(byte == 255u ? __uint_as_float(0x7FC00000u) : f[i]);
-    store_pack<T, E>(out + p.row * ldo + p.col, o, p.live);
+    for (int u = 0; u < U; ++u) {
+        in[u] = place_of<T, U>(p[u], u, steps, n_steps, cols);
+        if (in[u]) {
+            code[u] = reinterpret_cast<const W*>(codes)[p[u].lane];
+            e[u] = scales[p[u].lane / Lanes<T>::block];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (!in[u]) break;
+        const uint32_t w = code[u], byte = e[u];
+        const float scale = scale_value(byte == 255u ? 127u : byte);
+        float f[8];
+        values4<0>(w, scale, f[0], f[1]);
+        values4<1>(w, scale, f[2], f[3]);
+        if constexpr (E == 8) {
+            values4<2>(w, scale, f[4], f[5]);
+            values4<3>(w, scale, f[6], f[7]);
+        }
+        typename Pack<T, E>::vec o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = (T)(byte == 255u ? __uint_as_float(0x7FC00000u) : f[i]);
+        store_pack<T, E>(out + p[u].row * ldo + p[u].col, o, p[u].live);
+    }
 }
 
 // out = value of the codes (FN none) or dy * fn'(value).
-template <typename T, int FN>
+template <typename T, int FN, int U>
 __global__ __launch_bounds__(256) void act8_grad_kernel(T* out, uint64_t ldo, const T* dy, uint64_t ldy,
                                                         const uint8_t* codes, const uint8_t* scales, FastDiv steps,
                                                         uint32_t n_steps, uint32_t cols)
 {
     constexpr int E = Lanes<T>::E;
-    Place p;
-    if (!place_of<T>(p, steps, n_steps, cols)) return;
-    typename Pack<T, E>::vec g, o;
-    if constexpr (FN != NKMX_NONE) g = load_pack<T, E>(dy + p.row * ldy + p.col, p.live);
     typedef typename Word<E>::type W;
-    const W w = reinterpret_cast<const W*>(codes)[p.lane];
-    const float scale = scale_value(scales[p.lane / Lanes<T>::block]);
+    Place p[U];
+    bool in[U];
+    typename Pack<T, E>::vec g[U];
+    W code[U];
+    uint8_t e[U];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        uint32_t four;
-        if constexpr (E == 8) four = w[i / 4];
-        else four = w;
-        const float v = (float)(int8_t)(four >> (8 * (i & 3))) * scale;
-        if constexpr (FN != NKMX_NONE) o[i] = (T)(number(g[i]) * activation_slope<FN>(v));
-        else o[i] = (T)v;
+    for (int u = 0; u < U; ++u) {
+        in[u] = place_of<T, U>(p[u], u, steps, n_steps, cols);
+        if (in[u]) {
+            code[u] = reinterpret_cast<const W*>(codes)[p[u].lane];
+            e[u] = scales[p[u].lane / Lanes<T>::block];
+            if constexpr (FN != NKMX_NONE) g[u] = load_pack<T, E>(dy + p[u].row * ldy + p[u].col, p[u].live);
+        }
     }
-    store_pack<T, E>(out + p.row * ldo + p.col, o, p.live);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (!in[u]) break;
+        const float scale = scale_value(e[u]);
+        typename Pack<T, E>::vec o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            uint32_t four;
+            if constexpr (E == 8) four = code[u][i / 4];
+            else four = code[u];
+            const float v = (float)(int8_t)(four >> (8 * (i & 3))) * scale;
+            if constexpr (FN != NKMX_NONE) o[i] = (T)(number(g[u][i]) * activation_slope<FN>(v));
+            else o[i] = (T)v;
+        }
+        store_pack<T, E>(out + p[u].row * ldo + p[u].col, o, p[u].live);
+    }
 }
 
 // The transpose: blocks run down x's columns.  A workgroup of 8 waves takes 256 rows x 64 * CPL columns; a wave
-// takes 32 rows = one block of every column, a lane CPL = 2 (16-bit types, one 4-byte load a row) or 1 columns,
-// so a block never leaves its lane.  The codes cross LDS once, so that a column's 256 rows leave as 128
+// takes 32 rows = one block of every column, a lane CPL columns (one load of 4 or 8 bytes a row), so a block
+// never leaves its lane.  The codes cross LDS once, so that a column's 256 rows leave as 128
 // contiguous bytes: whole cache lines.
-template <typename T>
+template <typename T, int CPL>
 __global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x, uint64_t ldx, uint8_t* codes,
                                                                       uint8_t* scales, uint32_t rows, uint32_t cols,
                                                                       uint32_t steps, uint32_t col_tiles)
 {
-    constexpr int CPL = 4 / (int)sizeof(T);
     constexpr int TC = 64 * CPL;
     // 16-byte slots, 8 a column: slot s of column c lies at s ^ (c & 7), so that neither side collides in the banks
     __shared__ u32x4 image[TC * 8];
     __shared__ alignas(16) uint8_t bytes[TC * 8];
-    const uint32_t tile = blockIdx.x % col_tiles, band = blockIdx.x / col_tiles;
+    // each XCD takes a contiguous run of tiles: the cache lines that neighbours share are fetched into one L2
+    const uint32_t xcd = blockIdx.x & 7u, each = gridDim.x >> 3, more = gridDim.x & 7u;
+    const uint32_t t = xcd * each + min(xcd, more) + (blockIdx.x >> 3), tile = t % col_tiles, band = t / col_tiles;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t r0 = band * 256 + wave * 32, c0 = tile * TC + lane * CPL;
     const int live = (int)min((uint32_t)32, rows > r0 ? rows - r0 : 0u);
@@ -1533,23 +1593,32 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     }
 }
 
-// Joins the parts of a split weight gradient, [parts][rows][cols] in the workspace, in order.
-__global__ __launch_bounds__(256) void join_parts_kernel(float* out, uint64_t ldo, const float* part, uint32_t parts,
-                                                         uint64_t part_stride, uint32_t rows, uint32_t cols,
-                                                         uint64_t ldp, uint32_t accumulate)
+// Joins the parts of a split weight gradient in order: dw, [parts][rows][ldp] in the workspace, and behind each part's
+// dw its db as a row of `rows` numbers.  Rows of the workspace are whole quads.
+__global__ __launch_bounds__(256) void join_parts_kernel(float* dw, uint64_t lddw, float* db, const float* part, uint32_t parts,
+                                                         uint64_t part_stride, uint32_t rows, uint32_t cols, uint64_t ldp,
+                                                         uint32_t accumulate)
 {
     const uint32_t per_row = (cols + 3) / 4;
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint64_t row = i / per_row;
-    if (row >= rows) return;
-    const uint32_t col = (uint32_t)(i % per_row) * 4;
-    const int64_t live = (int64_t)cols - (int64_t)col;
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p = 0; p < parts; ++p) {  // rows of the workspace are padded to whole quads
-        const f32x4 v = *reinterpret_cast<const f32x4*>(part + p * part_stride + row * ldp + col);
-        s = p ? s + v : v;
+    uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t quads = (uint64_t)rows * per_row;
+    float* o;
+    int64_t live;
+    if (i < quads) {
+        const uint64_t row = i / per_row;
+        const uint32_t col = (uint32_t)(i - row * per_row) * 4;
+        part += row * ldp + col;
+        o = dw + row * lddw + col;
+        live = (int64_t)cols - (int64_t)col;
+    } else {
+        i -= quads;
+        live = (int64_t)rows - (int64_t)(4 * i);
+        if (db == nullptr || live <= 0) return;
+        part += rows * ldp + 4 * i;
+        o = db + 4 * i;
     }
-    float* o = out + row * ldo + col;
+    f32x4 s = *reinterpret_cast<const f32x4*>(part);
+    for (uint32_t p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(part + p * part_stride);
     if (accumulate) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1631,12 +1700,12 @@ struct Stream {
     FastDiv steps;
     uint32_t n_steps, cols, blocks;
 };
-template <typename T>
+template <typename T, int U>
 inline bool stream_of(Stream& s, uint64_t rows, uint64_t cols)
 {
     const uint64_t steps = steps_of(cols), total = rows * steps;  // both below 2^31
     if (total > 0xFFFFFFFFull) return false;
-    const uint64_t blocks = (total * Lanes<T>::step + 255) / 256;
+    const uint64_t blocks = (total * Lanes<T>::step + 256 * U - 1) / (256 * U);
     if (blocks > kMaxSize) return false;
     s = Stream{fast_div((uint32_t)steps), (uint32_t)total, (uint32_t)cols, (uint32_t)blocks};
     return true;
@@ -1803,15 +1872,28 @@ int nkmx_mx4_quantize(const void* x, int type, uint64_t rows, uint64_t cols, uin
     return for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
         if (transpose) {
-            constexpr uint64_t tc = 64 * (4 / sizeof(T));
-            const uint64_t tiles = (cols + tc - 1) / tc, bands = (rows + 255) / 256;
-            if (tiles * bands > kMaxSize) return NKMX_ERANGE;
-            return launch(mx4_quantize_transposed_kernel<T>, dim3((uint32_t)(tiles * bands)), 512, s, (const T*)x, ldx,
-                          codes, scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)steps_of(rows), (uint32_t)tiles);
+            // 8 bytes a lane and row from 1024 workgroups on (8192 x 4096 fp32 25.8 us against 28.6 with 4), 4 below
+            // (1024 x 1024 5.9 against 7.4)
+            const auto with = [&](auto bytes) -> int {
+                constexpr int CPL = decltype(bytes)::value / (int)sizeof(T);
+                const uint64_t tiles = (cols + 64 * CPL - 1) / (64 * CPL), bands = (rows + 255) / 256;
+                if (tiles * bands > kMaxSize) return NKMX_ERANGE;
+                return launch(mx4_quantize_transposed_kernel<T, CPL>, dim3((uint32_t)(tiles * bands)), 512, s, (const T*)x, ldx,
+                              codes, scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)steps_of(rows), (uint32_t)tiles);
+            };
+            if ((rows + 255) / 256 * ((cols * sizeof(T) + 511) / 512) >= 1024) return with(std::integral_constant<int, 8>{});
+            return with(std::integral_constant<int, 4>{});
         }
         Stream g;
-        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
-        return launch(mx4_quantize_kernel<T>, dim3(g.blocks), 256, s, (const T*)x, ldx, codes, scales, g.steps, g.n_steps,
+        // four pieces a lane where that still fills the chip: a pass that mostly reads wants more in flight than its
+        // lanes' 16 bytes (16384 x 8192 bf16 58 us with one, 55 with two, 52.5 with four; passes that write as much
+        // as they read lose by it)
+        if (!stream_of<T, 4>(g, rows, cols)) return NKMX_ERANGE;
+        if (g.blocks >= 1024)
+            return launch(mx4_quantize_kernel<T, 4>, dim3(g.blocks), 256, s, (const T*)x, ldx, codes, scales, g.steps,
+                          g.n_steps, g.cols);
+        stream_of<T, 1>(g, rows, cols);
+        return launch(mx4_quantize_kernel<T, 1>, dim3(g.blocks), 256, s, (const T*)x, ldx, codes, scales, g.steps, g.n_steps,
                       g.cols);
     });
 }
@@ -1828,8 +1910,8 @@ int nkmx_mx4_dequantize(void* out, int type, uint64_t rows, uint64_t cols, uint6
     return for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
         Stream g;
-        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
-        return launch(mx4_dequantize_kernel<T>, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, codes, scales,
+        if (!stream_of<T, 1>(g, rows, cols)) return NKMX_ERANGE;
+        return launch(mx4_dequantize_kernel<T, 1>, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, codes, scales,
                       g.steps, g.n_steps, g.cols);
     });
 }
@@ -1908,14 +1990,14 @@ int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint
     return for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
         Stream g;
-        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
+        if (!stream_of<T, 1>(g, rows, cols)) return NKMX_ERANGE;
         const auto with = [&](auto kernel) {
             return launch(kernel, dim3(g.blocks), 256, (hipStream_t)stream, (const T*)x, ldx, (T*)y, ldy, codes, scales,
                           g.steps, g.n_steps, g.cols);
         };
-        if (fn == NKMX_GELU) return with(act8_save_kernel<T, NKMX_GELU>);
-        if (fn == NKMX_SILU) return with(act8_save_kernel<T, NKMX_SILU>);
-        return with(act8_save_kernel<T, NKMX_NONE>);
+        if (fn == NKMX_GELU) return with(act8_save_kernel<T, NKMX_GELU, 1>);
+        if (fn == NKMX_SILU) return with(act8_save_kernel<T, NKMX_SILU, 1>);
+        return with(act8_save_kernel<T, NKMX_NONE, 1>);
     });
 }
 
@@ -1934,14 +2016,14 @@ static int act8_read(void* out, const void* dy, int type, int fn, uint64_t rows,
     return for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
         Stream g;
-        if (!stream_of<T>(g, rows, cols)) return NKMX_ERANGE;
+        if (!stream_of<T, 1>(g, rows, cols)) return NKMX_ERANGE;
         const auto with = [&](auto kernel) {
             return launch(kernel, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, (const T*)dy, lddy, codes,
                           scales, g.steps, g.n_steps, g.cols);
         };
-        if (fn == NKMX_GELU) return with(act8_grad_kernel<T, NKMX_GELU>);
-        if (fn == NKMX_SILU) return with(act8_grad_kernel<T, NKMX_SILU>);
-        return with(act8_grad_kernel<T, NKMX_NONE>);
+        if (fn == NKMX_GELU) return with(act8_grad_kernel<T, NKMX_GELU, 1>);
+        if (fn == NKMX_SILU) return with(act8_grad_kernel<T, NKMX_SILU, 1>);
+        return with(act8_grad_kernel<T, NKMX_NONE, 1>);
     });
 }
 
@@ -2005,15 +2087,10 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
                                                    stride, s);
     }));
     if (!split) return NKMX_OK;
-    const auto join = [&](float* out, uint64_t ldo, const float* from, uint64_t rows, uint64_t cols, uint64_t ldp) -> int {
-        const uint64_t blocks = (rows * ((cols + 3) / 4) + 255) / 256;
-        if (blocks > kMaxSize) return NKMX_ERANGE;
-        return launch(join_parts_kernel, dim3((uint32_t)blocks), 256, s, out, ldo, from, (uint32_t)p.parts, p.part_floats,
-                      (uint32_t)rows, (uint32_t)cols, ldp, accumulate ? 1u : 0u);
-    };
-    if (k) NKMX_TRY(join(dw, lddw, part, n, k, p.ldp));
-    if (db) NKMX_TRY(join(db, n, part + n * p.ldp, 1, n, n));
-    return NKMX_OK;
+    const uint64_t quads = n * ((k + 3) / 4) + (db ? (n + 3) / 4 : 0), blocks = (quads + 255) / 256;
+    if (blocks > kMaxSize) return NKMX_ERANGE;
+    return launch(join_parts_kernel, dim3((uint32_t)blocks), 256, s, dw, lddw, db, part, (uint32_t)p.parts, p.part_floats,
+                  (uint32_t)n, (uint32_t)k, p.ldp, accumulate ? 1u : 0u);
 }
 
 }  // extern "C"
