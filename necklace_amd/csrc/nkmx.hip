@@ -1346,9 +1346,9 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
 // (16 lanes read 4 tokens x 16 columns and get 4 tokens of one column each).  A row is TN / 32 pieces of 64 bytes; piece
 // c of token t lies at c ^ (t & 3), so that the four tokens that are read together do not meet in the banks.
 //
-// Order of a stage, whose loads count against each other: the codes of the stage after the next are loaded when those
-// of the next one have arrived, the next stage's dy just before them; at the end only the codes may still be on
-// their way.
+// A stage first asks for the next one's dy and the codes of the one after, then turns the codes that it was given into
+// the next stage's operand while its instructions run; the barrier comes before its last 16 tokens, whose
+// instructions cover the first reads of the next stage.
 template <int TN, int TK, int WN, int WK>
 __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_kernel(
     float* dw, uint64_t lddw, float* db, const bf16* dy, uint64_t lddy, const uint8_t* codes, const uint8_t* scales,
@@ -1469,17 +1469,20 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     };
 
     bf16x8 a[FN], b[2][FK];
-    // The 16 tokens h of a stage.  An operand is read for the next 16 as soon as it has been used; the instructions of
-    // what `work` adds and the LDS reads go between the matrix instructions.
-    const auto tokens = [&](int buf, auto index, auto work) NKMX_INLINE {
-        constexpr int h = decltype(index)::value;
-        if constexpr (h + 1 < GROUPS) take_b(b[(h + 1) & 1], buf, h + 1);
+    // The 16 tokens h of a stage.  An operand is read for the next 16 as soon as it has been used (READS; after the last of
+    // a stage: the next stage's first, in the other buffer); those reads and the instructions of what `work` adds go
+    // between the matrix instructions.
+    const auto tokens = [&](int buf, auto index, auto reads, auto work) NKMX_INLINE {
+        constexpr int h = decltype(index)::value, then = (h + 1) % GROUPS;
+        constexpr bool READS = decltype(reads)::value;
+        const int from = then ? buf : buf ^ 1;
+        if constexpr (READS) take_b(b[(h + 1) & 1], from, then);
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
 #pragma unroll
             for (int j = 0; j < FK; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[h & 1][j], acc[i][j], 0, 0, 0);
-            if constexpr (h + 1 < GROUPS) take_a(a[i], buf, h + 1, i);
+            if constexpr (READS) take_a(a[i], from, then, i);
         }
         work();
 #pragma unroll
@@ -1490,6 +1493,11 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
             __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // an LDS write
         }
         __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto begin = [&](int buf) NKMX_INLINE {
+        take_b(b[0], buf, 0);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) take_a(a[i], buf, 0, i);
     };
     typedef std::integral_constant<int, 0> H0;
     typedef std::integral_constant<int, 1> H1;
@@ -1502,44 +1510,36 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
         const auto stage = [&](uint32_t s, int buf, auto more) NKMX_INLINE {
             constexpr int MORE = decltype(more)::value;
             constexpr bool TURNS = MORE > 0 && XWAVES == WAVES;
-            take_b(b[0], buf, 0);
-#pragma unroll
-            for (int i = 0; i < FN; ++i) take_a(a[i], buf, 0, i);
-            __builtin_amdgcn_sched_barrier(0);
-            tokens(buf, H0{}, [] {});
-            if constexpr (decltype(sums)::value) add_up(buf);
+            typedef std::integral_constant<bool, true> Reads;
             if constexpr (MORE > 0) {
-                if constexpr (XWAVES == WAVES) {
-                    // (as assembly, or the moves, and with them the wait for the loads, go to the stage's beginning)
-                    asm volatile("v_mov_b32 %0, %1" : "=v"(now.e) : "v"(next.e));
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) asm volatile("v_mov_b32 %0, %1" : "=v"(now.q[i]) : "v"(next.q[i]));
-                    spread_scales(now.e, scale);
-                    fetch_d(s + 1, buf ^ 1);
+                fetch_d(s + 1, buf ^ 1);
+                if constexpr (TURNS) {
                     if constexpr (MORE > 1) fetch_x(next, s + 2);
-                } else {
-                    fetch_d(s + 1, buf ^ 1);
-                    if (has_x) {
-                        fetch_x(now, s + 1);
-                        spread_scales(now.e, scale);
+                    spread_scales(now.e, scale);
+                } else if (has_x) {
+                    fetch_x(now, s + 1);
+                    spread_scales(now.e, scale);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) put_x(now, scale, buf ^ 1, j);
-                    }
+                    for (int j = 0; j < 4; ++j) put_x(now, scale, buf ^ 1, j);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (decltype(sums)::value) add_up(buf);
+            __builtin_amdgcn_sched_barrier(0);
             const auto turn = [&](int from, int to) NKMX_INLINE {
                 if constexpr (TURNS) {
 #pragma unroll
                     for (int j = from; j < to; ++j) put_x(now, scale, buf ^ 1, j);
                 }
             };
-            tokens(buf, H1{}, [&]() NKMX_INLINE { turn(0, 2); });
-            tokens(buf, H2{}, [&]() NKMX_INLINE { turn(0, 0); });
-            tokens(buf, H3{}, [&]() NKMX_INLINE { turn(2, 4); });
-            // dy has arrived when no more than the 9 loads of codes behind it are on their way (fewer, to be safe)
-            if constexpr (TURNS && MORE > 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            tokens(buf, H0{}, Reads{}, [&]() NKMX_INLINE { turn(0, 1); });
+            tokens(buf, H1{}, Reads{}, [&]() NKMX_INLINE { turn(1, 2); });
+            tokens(buf, H2{}, Reads{}, [&]() NKMX_INLINE { turn(2, 4); });
+            // This stage has been read and the next one is there: its codes turned, its dy arrived when no more than the 9
+            // loads of codes behind it are on their way (fewer, to be safe).
+            if constexpr (TURNS && MORE > 1) arrived<4>();
             else arrived();
+            tokens(buf, H3{}, std::integral_constant<bool, (MORE > 0)>{}, [] {});
+            if constexpr (TURNS && MORE > 1) now = next;
         };
         const uint32_t fast = max(first, min(last, safe / BT));  // stages of whole tiles
         if (first < fast) {
@@ -1549,9 +1549,10 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
                 spread_scales(now.e, scale);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) put_x(now, scale, 0, j);
-                if (XWAVES == WAVES && first + 1 < fast) fetch_x(next, first + 1);
+                if (XWAVES == WAVES && first + 1 < fast) fetch_x(now, first + 1);
             }
             arrived();
+            begin(0);
             int buf = 0;
             for (uint32_t s = first; s + 2 < fast; ++s, buf ^= 1) stage(s, buf, std::integral_constant<int, 2>{});
             if (first + 1 < fast) {
@@ -1570,6 +1571,7 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
                 for (int j = 0; j < 4; ++j) put_x(now, scale, 0, j);
             }
             arrived();
+            begin(0);
             stage(s, 0, std::integral_constant<int, 0>{});
         }
     };
