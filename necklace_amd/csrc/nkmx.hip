@@ -628,7 +628,8 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_
 {
     __shared__ float sums[kRowsWaves][MT * NT * 256];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+    const uint32_t col_blocks = (n + 16 * NT - 1) / (16 * NT);
+    const uint32_t n0 = blockIdx.x % col_blocks * (16 * NT), m0 = blockIdx.x / col_blocks * (16 * MT);
     const u32x4 *pa[MT], *pb[NT];
     const uint32_t *qa[MT], *qb[NT];
 #pragma unroll
@@ -1131,9 +1132,10 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
     const int x_slot0 = (wave - XW) * 64 / CX, x_slot = x_slot0 + lane / CX, x_col = (lane % CX) * 4;
     const uint32_t pitch = steps * kStep, pitch_s = steps * 4, col_x = tc * TK + x_col;
     const uint32_t safe = safe_tokens(t_rows, n, (tr + 1) * TN, lddy, pitch, (tc + 1) * TK);
-    const uint32_t at_d = (uint32_t)(lane / CD) * 8 * (uint32_t)lddy * sizeof(T) + d_col * sizeof(T);
-    const uint32_t at_x = (lane / CX) * 8 * pitch + x_col;
-    const uint32_t at_s = ((lane / CX) * 8 + (lane & 7)) * pitch_s + x_col / 32;
+    typedef std::conditional_t<CD >= 64, uint32_t, uint64_t> At;  // lanes of one row group, or of several rows apart
+    const At at_d = (At)(lane / CD) * 8 * (At)lddy * sizeof(T) + d_col * sizeof(T);
+    const At at_x = (At)(lane / CX) * 8 * pitch + x_col;
+    const At at_s = (At)((lane / CX) * 8 + (lane & 7)) * pitch_s + x_col / 32;
 
     // Stages up to `safe` load whole tiles; the others element by element, with zeros past the ends.
     typename Pack<T, 4>::vec d[8];
@@ -1376,8 +1378,9 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     const int x_slot0 = wave * 64 / CX, x_slot = x_slot0 + lane / CX, x_col = (lane % CX) * 4;
     const uint32_t pitch = steps * kStep, pitch_s = steps * 4, col_x = tc * TK + x_col, ld2 = (uint32_t)lddy * 2;
     const uint32_t safe = safe_tokens(t_rows, n, (tr + 1) * TN, lddy, pitch, (tc + 1) * TK);
-    const uint32_t at_x = (lane / CX) * 8 * pitch + x_col;
-    const uint32_t at_s = ((lane / CX) * 8 + (lane & 7)) * pitch_s + x_col / 32;
+    typedef std::conditional_t<CX >= 64, uint32_t, uint64_t> At;  // lanes of one row group, or of several rows apart
+    const At at_x = (At)(lane / CX) * 8 * pitch + x_col;
+    const At at_s = (At)((lane / CX) * 8 + (lane & 7)) * pitch_s + x_col / 32;
 
     // Stages up to `safe` load whole tiles; the others element by element, with zeros past the ends.
     const auto row_of = [&](int load) NKMX_INLINE { return wave * ROWS + load * RP + lane / LR; };
@@ -1752,8 +1755,9 @@ inline int launch_rows(T* y, uint64_t ldy, const T* x, uint64_t ldx, const uint8
                        const uint8_t* cb, const uint8_t* sb, const T* bias, uint64_t m, uint64_t n, uint64_t k,
                        hipStream_t s)
 {
-    const dim3 grid((uint32_t)((n + 16 * NT - 1) / (16 * NT)), (uint32_t)((m + 16 * MT - 1) / (16 * MT)));
-    return launch(mx4_rows_kernel<T, MT, NT, FUSED>, grid, 64 * kRowsWaves, s, y, ldy, x, ldx, ca, sa, cb, sb, bias,
+    const uint64_t blocks = ((n + 16 * NT - 1) / (16 * NT)) * ((m + 16 * MT - 1) / (16 * MT));
+    if (blocks > kMaxSize) return NKMX_ERANGE;
+    return launch(mx4_rows_kernel<T, MT, NT, FUSED>, dim3((uint32_t)blocks), 64 * kRowsWaves, s, y, ldy, x, ldx, ca, sa, cb, sb, bias,
                   (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)steps_of(k));
 }
 
@@ -1804,6 +1808,9 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
 {
     const auto tiles = [&](uint64_t side) { return ((n + side - 1) / side) * ((k + side - 1) / side); };
     WgradPlan p = {};
+    // Tiles of 256 where they, cut along 1024 tokens, give every CU one; else of 128 where those, cut along 512, give
+    // every second CU one; else of 64 (bf16, us with tiles of 256 / 128 / 64): 16384 x 1024 x 1024 56 / 70 / 88, 2048 x 4096 x
+    // 4096 74 / 94 / 152, 4096 x 1024 x 1024 32 / 28 / 31, 8192 x 512 x 512 30 / 23 / 25, 512 x 1024 x 1024 21 / 12 / 9.6
     p.side = tiles(256) * ((t + 1023) / 1024) >= 256 ? 256 : (tiles(128) * ((t + 511) / 512) >= 128 ? 128 : 64);
     const uint64_t bt = p.side == 256 && type != NKMX_BF16 ? 32 : 64;
     const uint64_t stages = (t + bt - 1) / bt, count = tiles(p.side);

@@ -8,8 +8,8 @@ necklace_amd.cuda.mx.
                                    the rounding is treated as the identity (straight through)
     Mx4Weight(weight)              the codes alone, laid out once: .linear(x, bias) for serving
 
-x is float32, bfloat16 or float16 on the GPU, [..., in]; weight [out, in] and bias [out] of the same type.  Gradients
-have their tensor's type; the weight gradient is summed in fp32 whatever that is.  The calls run on torch's current
+x is float32, bfloat16 or float16 on the GPU, [..., in]; weight [out, in] and bias [out] of the same type (autocast does
+not change them).  Gradients have their tensor's type; the weight gradient is summed in fp32 whatever that is.  The calls run on torch's current
 stream and can be captured into a graph.  A backward pass that is captured has to be the first use of its leaves'
 gradients on that stream (torch's own rule): take them with `torch.autograd.grad`, or let no eager graph of the same
 leaves live during the capture.  Second derivatives are not available.
@@ -18,6 +18,11 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ...cuda import mx
+
+
+def _as_given():
+    """Types stay what the caller brought, inside an autocast region too."""
+    return torch.autocast("cuda", enabled=False)
 
 
 def _rows(t):
@@ -68,14 +73,16 @@ class _Act8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias):
         ctx.saved_x = ctx.needs_input_grad[1]
         ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
-        return torch.nn.functional.linear(x, weight, bias)
+        with _as_given():
+            return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         weight, *packed = ctx.saved_tensors
         dy = _rows(dy)
-        dx = dy @ weight if ctx.needs_input_grad[0] else None
+        with _as_given():
+            dx = dy @ weight if ctx.needs_input_grad[0] else None
         c, s = packed if ctx.saved_x else (None, None)
         dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return dx, dw, db
@@ -156,7 +163,7 @@ class Mx4Weight:
         """mx4(x) W^T (+ bias), [..., in] -> [..., out]; for use without gradients."""
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError("Mx4Weight.linear has no gradient: use mx4_linear, or torch.no_grad()")
-        if x.shape[-1] != self.shape[1]:
+        if x.dim() < 1 or x.shape[-1] != self.shape[1]:
             raise ValueError(f"x {tuple(x.shape)} does not fit the weight {self.shape}")
         x = _rows(x)
         y = torch.empty(*x.shape[:-1], self.shape[0], dtype=x.dtype, device=x.device)

@@ -324,3 +324,36 @@ def test_checkpoints_behind_four_gigabytes():
     assert_within(dw, np.tile(x64.sum(0), (3, 1)), 2.0 ** -22 * np.abs(x64).sum(0))
     mx.cu_fn_act8_load_e(x, c, s)
     assert np.array_equal(f64(x[-2:]), x64) and not x[:-2].any()
+
+
+@pytest.mark.parametrize("dtype,ld", [(torch.bfloat16, 1 << 24), (torch.float32, 1 << 26)], ids=["bfloat16", "float32"])
+def test_wgrad_of_gradients_whose_rows_lie_far_apart(dtype, ld):
+    """Rows of dy whose distances within a tile pass 2^31 and 2^32 bytes."""
+    t, n, k = 150, 70, 40
+    wide = torch.empty(t, ld, dtype=dtype, device="cuda")
+    dy = wide[:, 1000:1000 + n]
+    dy.copy_(values(4, t, n, dtype))
+    c, s, x = packed8(values(5, t, k, dtype))
+    dw, db = torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+    mx.cu_fn_act8_wgrad_e(dw, dy, c, s, DB=db)
+    d64 = f64(dy)
+    bound_w, bound_b = wgrad_bounds(d64, x, t, dtype)
+    assert_within(dw, matmul64(d64.T, x), bound_w, "dw")
+    assert_within(db, d64.sum(0), bound_b, "db")
+
+
+@pytest.mark.parametrize("left", [0, 1, 2, 3])
+@pytest.mark.parametrize("t,n,k", [(200, 130, 140), (3000, 300, 130), (9000, 520, 520)])
+def test_wgrad_of_bf16_gradients_at_any_start(t, n, k, left):
+    """Even starts and leading dimensions take dy to LDS as it lies in memory, odd ones through registers."""
+    for more in (0, 1):
+        wide = torch.full((t, n + left + 2 + more), float("nan"), dtype=torch.bfloat16, device="cuda")
+        dy = wide[:, left:left + n]
+        dy.copy_(values(t, t, n, torch.bfloat16, 0.1))
+        c, s, x = packed8(values(7, t, k, torch.bfloat16))
+        dw, db = torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+        mx.cu_fn_act8_wgrad_e(dw, dy, c, s, DB=db)
+        d64 = f64(dy)
+        bound_w, bound_b = wgrad_bounds(d64, x, t, torch.bfloat16)
+        assert_within(dw, matmul64(d64.T, x), bound_w, "dw")
+        assert_within(db, d64.sum(0), bound_b, "db")

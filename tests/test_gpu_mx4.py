@@ -264,3 +264,29 @@ def test_codes_behind_four_gigabytes():
     want = ref.mx4_decode(c[-2:].cpu().numpy(), s[-2:].cpu().numpy(), cols)
     assert np.array_equal(f64(x[-2:]), want)
     assert not x[:-2].any()
+
+
+def test_a_contracted_length_beyond_the_tiles_reach():
+    """More than 2^24 columns and more rows than the smallest kernel takes: codes that are zero but for a few columns."""
+    m, n, k = 40, 2064, (1 << 24) + 300
+    steps = ref.steps_of(k)
+    ca, sa = torch.zeros(m, steps * 64, dtype=torch.uint8, device="cuda"), torch.full((m, steps * 4), 127, dtype=torch.uint8, device="cuda")
+    cb, sb = torch.zeros(n, steps * 64, dtype=torch.uint8, device="cuda"), torch.full((n, steps * 4), 127, dtype=torch.uint8, device="cuda")
+    a, b = np.zeros((m, 6)), np.zeros((n, 6))
+    rng = np.random.default_rng(1)
+    for i, col in enumerate((0, 4097, 1 << 20, (1 << 24) - 1, 1 << 24, k - 1)):
+        for codes, vals in ((ca, a), (cb, b)):
+            c = rng.integers(0, 16, codes.shape[0])
+            codes[:, col // 2] |= torch.from_numpy((c << (4 * (col % 2))).astype(np.uint8)).cuda()
+            vals[:, i] = ref.GRID[c & 7] * np.where(c & 8, -1, 1)
+    y = torch.empty(m, n, device="cuda")
+    mx.cu_fn_mx4_matmul_e(y, ca, sa, cb, sb)
+    assert np.array_equal(f64(y), a @ b.T)  # six products of at most 36: exact
+
+
+def test_many_rows_without_columns():
+    m = 3_000_000
+    bias = torch.arange(3.0, device="cuda")
+    y = torch.full((m, 3), 7.0, device="cuda")
+    mx.cu_fn_mx4_matmul_e(y, *mx.mx4_empty(m, 0), *mx.mx4_empty(3, 0), bias=bias)
+    assert torch.equal(y, bias.expand(m, 3))

@@ -155,6 +155,16 @@ def test_refusals():
         torch.autograd.grad(g.sum(), x)
 
 
+def test_autocast_does_not_change_types():
+    x, w = torch.randn(4, 8, device="cuda", requires_grad=True), torch.randn(5, 8, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for layer in (ptmx.act8_linear, ptmx.mx4_linear):
+            y = layer(x, w)
+            assert y.dtype == torch.float32
+            dx, dw = torch.autograd.grad(y.sum(), (x, w))
+            assert dx.dtype == dw.dtype == torch.float32
+
+
 # ---- together
 
 def mlp(x, w1, b1, w2, mx4):
