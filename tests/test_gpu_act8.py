@@ -357,3 +357,23 @@ def test_wgrad_of_bf16_gradients_at_any_start(t, n, k, left):
         bound_w, bound_b = wgrad_bounds(d64, x, t, torch.bfloat16)
         assert_within(dw, matmul64(d64.T, x), bound_w, "dw")
         assert_within(db, d64.sum(0), bound_b, "db")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name)
+def test_wgrad_of_a_few_tiles_more_than_cus(dtype):
+    """258 tiles of 256: t is cut so that the rounds come out evenly."""
+    t, n, k = 3000, 257, 32900
+    assert mx.act8_wgrad_workspace(dtype, t, n, k) >= 2 * 4 * n * k
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(t, k, device="cuda", generator=g)
+    c, s = mx.act8_empty(t, k)
+    mx.cu_fn_act8_save_e(x, c, s)
+    mx.cu_fn_act8_load_e(x, c, s)
+    dy = torch.randn(t, n, device="cuda", generator=g).to(dtype)
+    dw, db = torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+    mx.cu_fn_act8_wgrad_e(dw, dy, c, s, DB=db)
+    d64, x64 = dy.double().t().contiguous(), x.double()
+    parts = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[dtype]
+    bound = (16 + parts * t / 16 + 257) * 2.0 ** -23 * (d64.abs() @ x64.abs())
+    assert bool(((dw.double() - d64 @ x64).abs() <= bound).all())
+    assert bool(((db.double() - d64.sum(1)).abs() <= (t / 4 + 16 + 257) * 2.0 ** -24 * d64.abs().sum(1)).all())
