@@ -86,7 +86,8 @@ uint64_t nkmx_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k);
 
 /*
  * x -> act8 codes of x, and y = fn(x) of the same type unless fn is NKMX_NONE (then y is NULL).  fn is
- * taken of x itself, not of its codes.  y may be x (with the same leading dimension).
+ * taken of x itself, not of its codes; gelu by a formula that is within 7.5e-7 of the normal
+ * distribution function, in fp32.  y may be x (with the same leading dimension).
  */
 int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint64_t cols, uint64_t ldx, uint64_t ldy,
                    uint8_t* codes, uint8_t* scales, void* stream);
@@ -102,8 +103,9 @@ int nkmx_act8_grad(void* dx, const void* dy, int type, int fn, uint64_t rows, ui
 /*
  * dw[j, c] = (accumulate ? dw[j, c] : 0) + sum over i of dy[i, j] * x^[i, c] for dy [t, n] of `type` and x
  * [t, k] in act8; dw is fp32 [n, k].  db (fp32 [n], may be NULL) gets the sums of dy's columns the same
- * way.  Every product is exact and the sums are fp32 for all three types.  The result does not depend
- * on timing.  `workspace`: nkmx_act8_wgrad_workspace bytes on a 16-byte boundary, NULL if that is 0.
+ * way.  Every product is exact and the sums are fp32 for all three types (an fp32 dy keeps all its bits
+ * from 2^-110 up).  The result does not depend on timing.  `workspace`: nkmx_act8_wgrad_workspace
+ * bytes on a 16-byte boundary, NULL if that is 0.
  */
 int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, uint64_t n, uint64_t k, uint64_t lddw,
                     uint64_t lddy, const uint8_t* codes, const uint8_t* scales, int accumulate, void* workspace,

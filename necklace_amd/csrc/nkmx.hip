@@ -309,6 +309,8 @@ __device__ __forceinline__ uint32_t codes4(V v, float scale)  // N = 4 or 8 valu
     return w;
 }
 
+// s + 17/32 bytes an element, as far as memory goes: 16384 x 8192 bf16 (340 MB) 50 .. 52.5 us = 6.5 .. 6.8 TB/s, where
+// a large copy runs at 6.9.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* x, uint64_t ldx, uint8_t* codes, uint8_t* scales,
                                                            FastDiv steps, uint32_t n_steps, uint32_t cols)
@@ -350,6 +352,8 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
     return ab | cd;
 }
 
+// 2 s + 33/32 bytes an element and, for gelu, some 40 vector instructions: 16384 x 4096 bf16 (338 MB) 54.6 us = 6.2 TB/s
+// with both nearly busy; two or four pieces a lane are slower (registers take waves away).
 template <typename T, int FN, int U>
 __global__ __launch_bounds__(256) void act8_save_kernel(const T* x, uint64_t ldx, T* y, uint64_t ldy, uint8_t* codes,
                                                         uint8_t* scales, FastDiv steps, uint32_t n_steps, uint32_t cols)
@@ -404,6 +408,7 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float& a, float
     b = v[1];
 }
 
+// The way back: 16384 x 8192 bf16 47 us = 7.2 TB/s.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(T* out, uint64_t ldo, const uint8_t* codes,
                                                              const uint8_t* scales, FastDiv steps, uint32_t n_steps,
@@ -442,7 +447,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(T* out, uint64_t ld
     }
 }
 
-// out = value of the codes (FN none) or dy * fn'(value).
+// out = value of the codes (FN none) or dy * fn'(value).  Bytes and bound as in act8_save_kernel: 16384 x 4096 bf16 gelu
+// 56 us = 6.0 TB/s.
 template <typename T, int FN, int U>
 __global__ __launch_bounds__(256) void act8_grad_kernel(T* out, uint64_t ldo, const T* dy, uint64_t ldy,
                                                         const uint8_t* codes, const uint8_t* scales, FastDiv steps,
@@ -485,7 +491,8 @@ __global__ __launch_bounds__(256) void act8_grad_kernel(T* out, uint64_t ldo, co
 // The transpose: blocks run down x's columns.  A workgroup of 8 waves takes 256 rows x 64 * CPL columns; a wave
 // takes 32 rows = one block of every column, a lane CPL columns (one load of 4 or 8 bytes a row), so a block
 // never leaves its lane.  The codes cross LDS once, so that a column's 256 rows leave as 128
-// contiguous bytes: whole cache lines.
+// contiguous bytes: whole cache lines.  Bound by memory: 8192 x 4096 fp32 (152 MB) 25.8 us = 5.9 TB/s; rows off the cache
+// lines, which neighbouring tiles then share, 8191 x 4097 30 us = 5.1 TB/s.
 template <typename T, int CPL>
 __global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x, uint64_t ldx, uint8_t* codes,
                                                                       uint8_t* scales, uint32_t rows, uint32_t cols,
@@ -554,8 +561,15 @@ __global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x
 // workgroup owns 16 NT rows of b and 16 MT of a; its 8 waves take a run of the steps of k each, straight from memory
 // into the operands of the 16 x 16 x 128 instruction (lane l holds row l % 16 and block l / 16 of the step, 16 bytes as
 // they are stored: four lanes read 64 bytes of a row, and the next step's load the rest of the cache line), four
-// steps at a time with one load of their scales.  The waves' sums are joined through LDS in wave order.  FUSED: a lane
-// quantizes its own block of 32 numbers of x in registers, with the arithmetic of mx4_quantize_kernel.
+// steps at a time, or two, with one load of their scales (16 lines again, for a sixteenth of the bytes).  The waves' sums
+// are joined through LDS in wave order.  FUSED: a lane quantizes its own block of 32 numbers of x in registers, with the
+// arithmetic of mx4_quantize_kernel.
+//
+// Rows of a x n x k, codes from HBM: 1 x 4096 x 1024 2.7 us (its 2.2 MB are 0.3): a launch and three memory latencies in a
+// chain; 1 x 8192 x 8192 (36 MB) 9.6; 1 x 28672 x 8192 (125 MB) 26.3 = 4.7 TB/s, 1 x 65536 x 4096 (143 MB) 26 = 5.5 TB/s,
+// 16 x 28672 x 8192 36: a's rows from L2 are as many bytes as b's then.  Loads of whole lines of 8 rows for two
+// instructions each gained nothing over this; k split over 4, 2 or 1 of the waves is slower from k = 4096 on (1 x 8192 x
+// 8192 12, 20, 33 us); more waves on a CU by fewer registers too.
 
 constexpr int kRowsWaves = 8;
 
@@ -627,7 +641,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_
                                                                    uint32_t k, uint32_t steps)
 {
     __shared__ float sums[kRowsWaves][MT * NT * 256];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const uint32_t col_blocks = (n + 16 * NT - 1) / (16 * NT);
     const uint32_t n0 = blockIdx.x % col_blocks * (16 * NT), m0 = blockIdx.x / col_blocks * (16 * MT);
     const u32x4 *pa[MT], *pb[NT];
@@ -646,12 +660,17 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_
     }
     f32x4 acc[MT][NT] = {};
     typedef u32x4 Loose __attribute__((aligned(4)));
+    typedef u32x2 Loose2 __attribute__((aligned(4)));
     const auto some = [&](uint32_t s, auto count) NKMX_INLINE {
         constexpr int N = decltype(count)::value;
         u32x4 a[N][MT], b[N][NT], ea[MT], eb[NT];
         const auto scales = [&](const uint32_t* q) NKMX_INLINE {
             if constexpr (N == 4) return *reinterpret_cast<const Loose*>(q + s);
-            else return u32x4{q[s], 0u, 0u, 0u};
+            if constexpr (N == 2) {
+                const u32x2 two = *reinterpret_cast<const Loose2*>(q + s);
+                return u32x4{two[0], two[1], 0u, 0u};
+            }
+            return u32x4{q[s], 0u, 0u, 0u};
         };
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -675,6 +694,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_
 #pragma unroll
                 for (int i = 0; i < N; ++i) a[i][t] = pa[t][(s + i) * 4];
             }
+            __builtin_amdgcn_sched_barrier(0);  // every load before the first wait: left alone the compiler saves registers
         }
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -699,6 +719,10 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(T* y, uint64_
     const uint32_t each = (steps + kRowsWaves - 1) / kRowsWaves, end = min(steps, (wave + 1) * each);
     uint32_t s = wave * each;
     for (; s + 4 <= end; s += 4) some(s, std::integral_constant<int, 4>{});
+    if (s + 2 <= end) {
+        some(s, std::integral_constant<int, 2>{});
+        s += 2;
+    }
     for (; s < end; ++s) some(s, std::integral_constant<int, 1>{});
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -732,6 +756,11 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t row_tiles, uint32_t
 // 16 bytes; slot s of row r lies at s ^ swizzle8(r), so that the 16 rows that are read together do not meet; a
 // load writes LDS in lane order, so the lanes' addresses carry the exchange.  The buffer's extent ends the rows: a
 // row past the matrix is not read, and its results are not stored.
+//
+// 8192 x 8192 x 8192: 270 us = 4.06 PFLOP/s in a row of calls, 281 .. 294 between other work; the instructions alone would
+// take 139.  With the loads to LDS left out 219: the rest is LDS, where a wave of 128 x 64 reads 6 operands for 8
+// instructions, and the wait at the one barrier of a stage.  Waves of 128 x 128 read less and take 290 (one a SIMD, nothing
+// runs while it waits); stages of 64 bytes through four buffers 345 (half lines).
 
 constexpr int kSpan = 4;  // steps whose scales are loaded at a time
 
@@ -997,6 +1026,9 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
 //
 // LDS: column c of a tile is BT tokens = BT / 8 slots; slot s lies at s ^ swizzle_t(c).  t is split over
 // blockIdx.y where there are few tiles; the parts are joined in order by a second kernel.
+//
+// Bound by the matrix instructions and the LDS traffic and turning between them: fp32 16384 x 4352 x 4096 1551 us, 1.13
+// PFLOP/s of bf16 products; 5001 x 1023 x 4097 (3 parts of 68 tiles: 204 of 256 CUs) 138 us and 11 to join.
 
 template <int SLOTS>
 __device__ __forceinline__ uint32_t swizzle_t(uint32_t c)
@@ -1351,6 +1383,10 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
 // A stage first asks for the next one's dy and the codes of the one after, then turns the codes that it was given into
 // the next stage's operand while its instructions run; the barrier comes before its last 16 tokens, whose
 // instructions cover the first reads of the next stage.
+//
+// 16384 x 4096 x 4096: 472 us = 1.16 PFLOP/s, where a large bf16 library product runs at 1.20 to 1.35; 16384 x 4096 x 1024 (4
+// parts of 64 tiles) 142 us, of which the parts' stores are some 15, and 13 to join.  The kernel above takes 173 there.  Waves
+// of 64 x 128, late waves, wave priorities and a touch of L2 two stages ahead were no faster.
 template <int TN, int TK, int WN, int WK>
 __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_kernel(
     float* dw, uint64_t lddw, float* db, const bf16* dy, uint64_t lddy, const uint8_t* codes, const uint8_t* scales,
@@ -1599,7 +1635,8 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
 }
 
 // Joins the parts of a split weight gradient in order: dw, [parts][rows][ldp] in the workspace, and behind each part's
-// dw its db as a row of `rows` numbers.  Rows of the workspace are whole quads.
+// dw its db as a row of `rows` numbers.  Rows of the workspace are whole quads.  4 parts of 4096 x 1024 (84 MB) 12 .. 13
+// us = 6.5 TB/s.
 __global__ __launch_bounds__(256) void join_parts_kernel(float* dw, uint64_t lddw, float* db, const float* part, uint32_t parts,
                                                          uint64_t part_stride, uint32_t rows, uint32_t cols, uint64_t ldp,
                                                          uint32_t accumulate)
@@ -1774,7 +1811,7 @@ inline int launch_tiles(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa
 // Which kernel, by counts of workgroups (us at m x n x k, codes from HBM):
 //   rows 16 x 16      up to 16 rows, and while there are at most 384 of them: 64 x 1024 x 4096 4.8 against 8.0 by tiles,
 //                     100 x 1024 x 1024 (448) 4.2 against 4.4, 200 x 1024 x 1024 (832) 6.6 against 4.4
-//   rows 32 x 32      up to 32 rows: 32 x 8192 x 8192 15.1 against 15.3 by tiles of 64, and 22.7 by rows of 16
+//   rows 32 x 32      up to 32 rows: 32 x 8192 x 8192 13.1 against 15.3 by tiles of 64, and 22.7 by rows of 16
 //   tiles 256         from 192 tiles: 4096^3 43 against 55 by tiles of 128; 2048 x 4096 x 4096 (128 tiles) 33 against 26
 //   tiles 128         from 192 tiles: 1024 x 4096 x 4096 17 against 22 by tiles of 64; 512 x 4096 x 4096 (128) 15 against
 //                     12.6; with four buffers while every workgroup has a CU of its own (512 x 8192 x 8192 30 against 41

@@ -290,3 +290,37 @@ def test_many_rows_without_columns():
     y = torch.full((m, 3), 7.0, device="cuda")
     mx.cu_fn_mx4_matmul_e(y, *mx.mx4_empty(m, 0), *mx.mx4_empty(3, 0), bias=bias)
     assert torch.equal(y, bias.expand(m, 3))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 16500, 4100), (16, 34000, 2000), (9, 4111, 16600)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=name)
+def test_few_rows_against_a_large_matrix(m, n, k, dtype):
+    """Two steps of k at a time, 33, 16 and 130 of them; a block of NaN stays in its row of b."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+
+    def made(rows, scale):
+        c, s = mx.mx4_empty(rows, k)
+        mx.cu_fn_mx4_quantize_e(torch.randn(rows, k, device="cuda", generator=g) * scale, c, s)
+        v = torch.empty(rows, k, device="cuda")
+        mx.cu_fn_mx4_dequantize_e(v, c, s)
+        return c, s, v.double()
+
+    ca, sa, a = made(m, 1.0)
+    cb, sb, b = made(n, 0.05)
+    y = torch.empty(m, n, dtype=dtype, device="cuda")
+    mx.cu_fn_mx4_matmul_e(y, ca, sa, cb, sb)
+    bt = b.t().contiguous()
+    want = a @ bt
+    assert_within(y, f64(want), product_bound_of(f64(a.abs() @ bt.abs()), f64(want), k, dtype), "matmul")
+    bad = [7, 15, n - 1]
+    sb[bad, 5] = 255
+    z = torch.empty_like(y)
+    mx.cu_fn_mx4_matmul_e(z, ca, sa, cb, sb)
+    assert bool(torch.isnan(z[:, bad]).all())
+    z[:, bad] = y[:, bad]
+    assert torch.equal(z, y)
+
+
+def product_bound_of(mags, want, k, dtype):
+    r = (128 + k / 64 + 8) * 2.0 ** -23 * mags
+    return r + half_step(dtype) * (np.abs(want) + r) + (2.0 ** -25 if dtype == torch.float16 else 0)
