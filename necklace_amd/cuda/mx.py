@@ -11,9 +11,9 @@ scale, rows are padded with zeros to whole steps of 128 columns.
   times the scale with a sign; `mx4_empty` makes the tensors;
 * act8: codes int8 [rows, steps * 128], whole numbers -127 .. 127 times the scale; `act8_empty`;
 * both: scales uint8 [rows, steps * 4], exponent + 127; 255 marks a block that held an infinity or a NaN: it decodes
-  to NaN.  The largest error is half a code's distance: 2^e / 2 for act8 (2^e for the largest magnitude of a block
-  where it rounds to 128), for mx4 a quarter of the value's own power of two, and a quarter of the value where it is
-  beyond 6 scales.
+  to NaN.  A value is off by at most half the distance of the codes around it: for act8 2^e / 2 (2^e where the
+  largest magnitude of a block would round to 128), for mx4 2^e / 4 below 2 scales, 2^e / 2 from there to 4, 2^e from
+  there to 6; beyond, where 6 is the last code, less than 2 * 2^e.
 
 Tensors of numbers are float32, bfloat16 or float16 and may be column ranges of wider matrices (any leading
 dimension, columns next to each other); more than two dimensions are taken as rows of the last one where that needs
