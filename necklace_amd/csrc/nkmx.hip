@@ -757,10 +757,11 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t row_tiles, uint32_t
 // load writes LDS in lane order, so the lanes' addresses carry the exchange.  The buffer's extent ends the rows: a
 // row past the matrix is not read, and its results are not stored.
 //
-// 8192 x 8192 x 8192: 270 us = 4.06 PFLOP/s in a row of calls, 281 .. 294 between other work; the instructions alone would
-// take 139.  With the loads to LDS left out 219: the rest is LDS, where a wave of 128 x 64 reads 6 operands for 8
-// instructions, and the wait at the one barrier of a stage.  Waves of 128 x 128 read less and take 290 (one a SIMD, nothing
-// runs while it waits); stages of 64 bytes through four buffers 345 (half lines).
+// 8192 x 8192 x 8192: 261 .. 275 us = 4.0 .. 4.2 PFLOP/s in a row of calls, 281 .. 294 between other work; the instructions
+// alone would take 139.  The same launch on codes of zeros takes 202: half of what is left is the clock, which falls
+// with the power that random operands take.  The rest is LDS, where a wave of 128 x 64 reads 6 operands for 8
+// instructions, and the wait at the one barrier of a stage.  Waves of 128 x 128 read a third less and take 267 .. 290 (one a
+// SIMD, nothing runs while it waits; 228 on zeros); stages of 64 bytes through four buffers 345 (half lines).
 
 constexpr int kSpan = 4;  // steps whose scales are loaded at a time
 
@@ -1385,8 +1386,10 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
 // instructions cover the first reads of the next stage.
 //
 // 16384 x 4096 x 4096: 472 us = 1.16 PFLOP/s, where a large bf16 library product runs at 1.20 to 1.35; 16384 x 4096 x 1024 (4
-// parts of 64 tiles) 142 us, of which the parts' stores are some 15, and 13 to join.  The kernel above takes 173 there.  Waves
-// of 64 x 128, late waves, wave priorities and a touch of L2 two stages ahead were no faster.
+// parts of 64 tiles) 138 us, of which the parts' stores are some 15, and 14 to join; the kernel above takes 177 and 14.  On
+// zeros both calls take a fifth less (376, and 122 with the join): the clock falls with the power of random operands, as for
+// the library.  Waves of 64 x 128, late waves, wave priorities, other orders of the tiles and a touch of L2 two stages
+// ahead were no faster.
 template <int TN, int TK, int WN, int WK>
 __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_kernel(
     float* dw, uint64_t lddw, float* db, const bf16* dy, uint64_t lddy, const uint8_t* codes, const uint8_t* scales,
