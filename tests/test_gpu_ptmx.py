@@ -343,3 +343,26 @@ def test_a_captured_training_step(mx4):
         g.replay()
         torch.cuda.synchronize()
         assert equal(got, step())
+
+
+@pytest.mark.parametrize("layer", [ptmx.act8_linear, ptmx.mx4_linear])
+@pytest.mark.parametrize("shape", [(0, 48), (3, 0, 48), (1, 48), (48,)], ids=str)
+def test_no_tokens_and_one_token(layer, shape):
+    x = torch.randn(shape, device="cuda").requires_grad_()
+    w = torch.randn(20, 48, device="cuda").requires_grad_()
+    b = torch.randn(20, device="cuda").requires_grad_()
+    y = layer(ptmx.act8_act(x, "silu"), w, b)
+    assert y.shape == shape[:-1] + (20,)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert dx.shape == x.shape and dw.shape == w.shape
+    tokens = x.numel() // 48
+    assert torch.equal(db, torch.full_like(db, tokens))
+    assert tokens or not dw.any()
+    assert ptmx.Mx4Weight(w).linear(x.detach()).shape == y.shape
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 48, device="cuda").requires_grad_()
+    dx, = torch.autograd.grad(ptmx.act8_act(x, "gelu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
