@@ -152,21 +152,25 @@ def _device(first, *others):
     return dev
 
 
-class _on_device:
-    """`with torch.cuda.device(index)` only when that is not the current one already."""
-    __slots__ = ("ctx",)
-
-    def __init__(self, index):
-        self.ctx = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+class _Here:
+    """`with` nothing."""
+    __slots__ = ()
 
     def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
+        pass
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            return self.ctx.__exit__(*exc)
-        return False
+        pass
+
+
+_HERE = _Here()
+# torch's accessor behind torch.cuda.current_device (0.06 us against 0.23); the documented route where it is absent
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _on_device(index):
+    """`torch.cuda.device(index)` only when that is not the current one already."""
+    return _HERE if index == _current_device() else torch.cuda.device(index)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -202,7 +206,7 @@ def _bias(bias, n, y):
     if not isinstance(bias, torch.Tensor):
         raise TypeError(f"bias: expected a torch tensor, got {type(bias).__name__}")
     _same_type("bias", bias, "Y", y.dtype)
-    if tuple(bias.shape) != (n,) or (n > 1 and bias.stride(0) != 1):
+    if bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
         raise ValueError(f"bias: expected {n} contiguous elements")
     return bias.data_ptr()
 
@@ -375,7 +379,7 @@ def cu_fn_act8_wgrad_e(DW, DY, C, S, DB=None, accumulate=False, workspace=None, 
     if DB is not None:
         if not isinstance(DB, torch.Tensor) or DB.dtype != torch.float32:
             raise TypeError("DB: expected a float32 tensor")
-        if tuple(DB.shape) != (n,) or (n > 1 and DB.stride(0) != 1):
+        if DB.shape != (n,) or (n > 1 and DB.stride(0) != 1):
             raise ValueError(f"DB: expected {n} contiguous elements")
         db = DB.data_ptr()
     dev = _device(DW, DY, C, S, DB)
