@@ -1383,7 +1383,8 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
 //
 // A stage first asks for the next one's dy and the codes of the one after, then turns the codes that it was given into
 // the next stage's operand while its instructions run; the barrier comes before its last 16 tokens, whose
-// instructions cover the first reads of the next stage.
+// instructions cover the first reads of the next stage.  Tiles of 64 have one instruction for each 16 tokens and are bound
+// by waiting: they read a stage's operands at once and ask for dy three stages ahead (0.62 us a stage against 0.86).
 //
 // 16384 x 4096 x 4096: 472 us = 1.16 PFLOP/s, where a large bf16 library product runs at 1.20 to 1.35; 16384 x 4096 x 1024 (4
 // parts of 64 tiles) 138 us, of which the parts' stores are some 15, and 14 to join; the kernel above takes 177 and 14.  On
@@ -1402,8 +1403,11 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     constexpr int PIECES = TN / 32, LR = TN / 8, RP = 64 / LR;          // of a row of dy; lanes of a row, rows of a load
     constexpr int ROWS = BT / WAVES, LOADS = ROWS / RP;                 // rows and loads of a wave
     constexpr int TURN = PIECES < 4 ? PIECES - 1 : 3;
-    static_assert(XWAVES <= WAVES && LOADS * RP == ROWS, "units and waves");
-    __shared__ u32x4 left[2][BT * TN / 8];
+    constexpr bool ALL_X = XWAVES == WAVES;
+    constexpr bool SHORT = FN * FK == 1;   // one instruction each: what counts is the chain of waits
+    constexpr int DEPTH = SHORT ? 4 : 2;   // buffers of dy
+    static_assert(XWAVES <= WAVES && LOADS * RP == ROWS && !(SHORT && ALL_X), "units and waves");
+    __shared__ u32x4 left[DEPTH][BT * TN / 8];
     __shared__ u32x4 right[2][TK * SLOTS];
 
     uint32_t tr, tc;
@@ -1413,7 +1417,7 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     const int wn = (wave / WAVES_K) * WN, wk = (wave % WAVES_K) * WK;
     const uint32_t stages = (t_rows + BT - 1) / BT;
     const uint32_t first = blockIdx.y * stages_each, last = min(stages, first + stages_each);
-    const bool has_x = XWAVES == WAVES || wave < XWAVES;
+    const bool has_x = ALL_X || wave < XWAVES;
     const int x_slot0 = wave * 64 / CX, x_slot = x_slot0 + lane / CX, x_col = (lane % CX) * 4;
     const uint32_t pitch = steps * kStep, pitch_s = steps * 4, col_x = tc * TK + x_col, ld2 = (uint32_t)lddy * 2;
     const uint32_t safe = safe_tokens(t_rows, n, (tr + 1) * TN, lddy, pitch, (tc + 1) * TK);
@@ -1444,6 +1448,10 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     };
     struct Unit {
         uint32_t q[8], e;  // codes of 8 tokens x 4 columns; scale byte of token lane % 8 (see the kernel above)
+    };
+    const auto settle = [&](Unit& u) NKMX_INLINE {
+        asm volatile("" : "+v"(u.q[0]), "+v"(u.q[1]), "+v"(u.q[2]), "+v"(u.q[3]), "+v"(u.q[4]), "+v"(u.q[5]), "+v"(u.q[6]),
+                     "+v"(u.q[7]), "+v"(u.e));
     };
     const auto fetch_x = [&](Unit& u, uint32_t stage) NKMX_INLINE {
         const uint32_t t = stage * BT + x_slot0 * 8;
@@ -1511,20 +1519,28 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     };
 
     bf16x8 a[FN], b[2][FK];
+    bf16x8 all_a[SHORT ? GROUPS : 1][FN], all_b[SHORT ? GROUPS : 1][FK];  // SHORT: a whole stage's operands
+    const auto take_all = [&](int lb, int rb) NKMX_INLINE {
+#pragma unroll
+        for (int h = 0; h < GROUPS; ++h) {
+            take_b(all_b[h], rb, h);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) take_a(all_a[h][i], lb, h, i);
+        }
+    };
     // The 16 tokens h of a stage.  An operand is read for the next 16 as soon as it has been used (READS; after the last of
     // a stage: the next stage's first, in the other buffer); those reads and the instructions of what `work` adds go
     // between the matrix instructions.
-    const auto tokens = [&](int buf, auto index, auto reads, auto work) NKMX_INLINE {
+    const auto tokens = [&](int from_left, int from_right, auto index, auto reads, auto work) NKMX_INLINE {
         constexpr int h = decltype(index)::value, then = (h + 1) % GROUPS;
         constexpr bool READS = decltype(reads)::value;
-        const int from = then ? buf : buf ^ 1;
-        if constexpr (READS) take_b(b[(h + 1) & 1], from, then);
+        if constexpr (READS) take_b(b[(h + 1) & 1], from_right, then);
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
 #pragma unroll
             for (int j = 0; j < FK; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[h & 1][j], acc[i][j], 0, 0, 0);
-            if constexpr (READS) take_a(a[i], from, then, i);
+            if constexpr (READS) take_a(a[i], from_left, then, i);
         }
         work();
 #pragma unroll
@@ -1537,6 +1553,7 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
         __builtin_amdgcn_sched_barrier(0);
     };
     const auto begin = [&](int buf) NKMX_INLINE {
+        if constexpr (SHORT) return take_all(buf, buf);
         take_b(b[0], buf, 0);
 #pragma unroll
         for (int i = 0; i < FN; ++i) take_a(a[i], buf, 0, i);
@@ -1546,62 +1563,98 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     typedef std::integral_constant<int, 2> H2;
     typedef std::integral_constant<int, 3> H3;
     const auto run = [&](auto sums) NKMX_INLINE {
-        Unit now, next;
+        Unit now, next;  // codes of the next stage and of the one after
         float scale[8];
-        // MORE: stages that follow and are loaded from this one, 2 (codes of the second, dy of the first), 1 or 0.
-        const auto stage = [&](uint32_t s, int buf, auto more) NKMX_INLINE {
-            constexpr int MORE = decltype(more)::value;
-            constexpr bool TURNS = MORE > 0 && XWAVES == WAVES;
+        // A stage with dy in left[lb], codes turned in right[rb].  NEXT: another one follows; LOAD_X: and one after that, whose
+        // codes are asked for; LOAD_D: dy of the stage DEPTH - 1 further on is.
+        const auto stage = [&](uint32_t s, int lb, int rb, auto load_d, auto load_x, auto has_next) NKMX_INLINE {
+            constexpr bool LOAD_D = decltype(load_d)::value, LOAD_X = decltype(load_x)::value, NEXT = decltype(has_next)::value;
             typedef std::integral_constant<bool, true> Reads;
-            if constexpr (MORE > 0) {
-                fetch_d(s + 1, buf ^ 1);
-                if constexpr (TURNS) {
-                    if constexpr (MORE > 1) fetch_x(next, s + 2);
-                    spread_scales(now.e, scale);
-                } else if (has_x) {
-                    fetch_x(now, s + 1);
-                    spread_scales(now.e, scale);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) put_x(now, scale, buf ^ 1, j);
-                }
+            const int next_lb = lb + 1 == DEPTH ? 0 : lb + 1;
+            // SHORT: the next stage's codes are waited for before anything new is asked for: the compiler counts the loads that may
+            // still be on their way, and those to LDS, which it does not know, would have to arrive as well
+            if constexpr (SHORT && NEXT) {
+                if (has_x) settle(now);
             }
-            if constexpr (decltype(sums)::value) add_up(buf);
+            if constexpr (LOAD_D) fetch_d(s + DEPTH - 1, lb ? lb - 1 : DEPTH - 1);
+            if constexpr (ALL_X) {
+                if constexpr (LOAD_X) fetch_x(next, s + 2);
+                if constexpr (NEXT) spread_scales(now.e, scale);
+            } else if (NEXT && has_x) {
+                if constexpr (LOAD_X) fetch_x(next, s + 2);
+                spread_scales(now.e, scale);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) put_x(now, scale, rb ^ 1, j);
+            }
+            if constexpr (decltype(sums)::value) add_up(lb);
+            if constexpr (SHORT) {
+#pragma unroll
+                for (int h = 0; h < GROUPS; ++h)
+#pragma unroll
+                    for (int i = 0; i < FN; ++i)
+#pragma unroll
+                        for (int j = 0; j < FK; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(all_a[h][i], all_b[h][j], acc[i][j], 0, 0, 0);
+                if constexpr (LOAD_D && LOAD_X) {
+                    if (has_x) arrived<(DEPTH - 2) * LOADS + (DEPTH - 1) * 8>();
+                    else arrived<(DEPTH - 2) * LOADS>();
+                } else {
+                    arrived();
+                }
+                if constexpr (NEXT) take_all(next_lb, rb ^ 1);
+                if constexpr (LOAD_X) now = next;
+                return;
+            }
             __builtin_amdgcn_sched_barrier(0);
             const auto turn = [&](int from, int to) NKMX_INLINE {
-                if constexpr (TURNS) {
+                if constexpr (ALL_X && NEXT) {
 #pragma unroll
-                    for (int j = from; j < to; ++j) put_x(now, scale, buf ^ 1, j);
+                    for (int j = from; j < to; ++j) put_x(now, scale, rb ^ 1, j);
                 }
             };
-            tokens(buf, H0{}, Reads{}, [&]() NKMX_INLINE { turn(0, 1); });
-            tokens(buf, H1{}, Reads{}, [&]() NKMX_INLINE { turn(1, 2); });
-            tokens(buf, H2{}, Reads{}, [&]() NKMX_INLINE { turn(2, 4); });
-            // This stage has been read and the next one is there: its codes turned, its dy arrived when no more than the 9
-            // loads of codes behind it are on their way (fewer, to be safe).
-            if constexpr (TURNS && MORE > 1) arrived<4>();
-            else arrived();
-            tokens(buf, H3{}, std::integral_constant<bool, (MORE > 0)>{}, [] {});
-            if constexpr (TURNS && MORE > 1) now = next;
+            tokens(lb, rb, H0{}, Reads{}, [&]() NKMX_INLINE { turn(0, 1); });
+            tokens(lb, rb, H1{}, Reads{}, [&]() NKMX_INLINE { turn(1, 2); });
+            tokens(lb, rb, H2{}, Reads{}, [&]() NKMX_INLINE { turn(2, 4); });
+            // This stage has been read and the next one is there: its codes turned, its dy arrived when no more than the loads
+            // that were asked for behind it are on their way: dy of DEPTH - 2 stages, and 9 loads of codes (8, to be safe) each
+            // and with its own.
+            if constexpr (LOAD_D && LOAD_X) {
+                if (has_x) arrived<(DEPTH - 2) * LOADS + (DEPTH - 1) * 8>();
+                else arrived<(DEPTH - 2) * LOADS>();
+            } else {
+                arrived();
+            }
+            tokens(next_lb, rb ^ 1, H3{}, std::integral_constant<bool, NEXT>{}, [] {});
+            if constexpr (LOAD_X) now = next;
         };
+        typedef std::true_type Yes;
+        typedef std::false_type No;
         const uint32_t fast = max(first, min(last, safe / BT));  // stages of whole tiles
         if (first < fast) {
-            fetch_d(first, 0);
+            for (uint32_t s = 0; s + 1 < DEPTH && first + s < fast; ++s) fetch_d(first + s, s);
             if (has_x) {
                 fetch_x(now, first);
                 spread_scales(now.e, scale);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) put_x(now, scale, 0, j);
-                if (XWAVES == WAVES && first + 1 < fast) fetch_x(now, first + 1);
+                if (first + 1 < fast) fetch_x(now, first + 1);
             }
             arrived();
             begin(0);
-            int buf = 0;
-            for (uint32_t s = first; s + 2 < fast; ++s, buf ^= 1) stage(s, buf, std::integral_constant<int, 2>{});
-            if (first + 1 < fast) {
-                stage(fast - 2, buf, std::integral_constant<int, 1>{});
-                buf ^= 1;
+            int lb = 0, rb = 0;
+            const auto on = [&]() NKMX_INLINE {
+                lb = lb + 1 == DEPTH ? 0 : lb + 1;
+                rb ^= 1;
+            };
+            uint32_t s = first;
+            for (; s + max(DEPTH - 1, 2) < fast; ++s, on()) stage(s, lb, rb, Yes{}, Yes{}, Yes{});
+            if constexpr (DEPTH > 2)
+                for (; s + 2 < fast; ++s, on()) stage(s, lb, rb, No{}, Yes{}, Yes{});
+            if (s + 1 < fast) {
+                stage(s, lb, rb, std::integral_constant<bool, DEPTH == 2>{}, No{}, Yes{});
+                on();
             }
-            stage(fast - 1, buf, std::integral_constant<int, 0>{});
+            stage(fast - 1, lb, rb, No{}, No{}, No{});
         }
 #pragma unroll 1
         for (uint32_t s = fast; s < last; ++s) {  // the last tokens
@@ -1614,7 +1667,7 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
             }
             arrived();
             begin(0);
-            stage(s, 0, std::integral_constant<int, 0>{});
+            stage(s, 0, 0, No{}, No{}, No{});
         }
     };
     if (db != nullptr && tc == 0) run(std::true_type{});
@@ -1663,7 +1716,15 @@ __global__ __launch_bounds__(256) void join_parts_kernel(float* dw, uint64_t ldd
         o = db + 4 * i;
     }
     f32x4 s = *reinterpret_cast<const f32x4*>(part);
-    for (uint32_t p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(part + p * part_stride);
+    uint32_t p = 1;
+    for (; p + 4 <= parts; p += 4) {  // four loads on their way at a time, added in order
+        f32x4 v[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(part + (p + j) * part_stride);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) s += v[j];
+    }
+    for (; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(part + p * part_stride);
     if (accumulate) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1848,10 +1909,13 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
 {
     const auto tiles = [&](uint64_t side) { return ((n + side - 1) / side) * ((k + side - 1) / side); };
     WgradPlan p = {};
-    // Tiles of 256 where they, cut along 1024 tokens, give every CU one; else of 128 where those, cut along 512, give
-    // every second CU one; else of 64 (bf16, us with tiles of 256 / 128 / 64): 16384 x 1024 x 1024 56 / 70 / 88, 2048 x 4096 x
-    // 4096 74 / 94 / 152, 4096 x 1024 x 1024 32 / 28 / 31, 8192 x 512 x 512 30 / 23 / 25, 512 x 1024 x 1024 21 / 12 / 9.6
-    p.side = tiles(256) * ((t + 1023) / 1024) >= 256 ? 256 : (tiles(128) * ((t + 511) / 512) >= 128 ? 128 : 64);
+    // Tiles of 256 where they, cut along 1024 tokens, give every CU one (bf16, us with tiles of 256 / 128 / 64: 16384 x 1024
+    // x 1024 56 / 70 / 88, 2048 x 4096 x 4096 74 / 94 / 152).  Else of 128 where nearly every CU has one without a cut (500 x
+    // 2000 x 2000 bf16 20 against 25 with tiles of 64, fp32 27 against 33; 1000 x 1000 x 1000 bf16 23 against 16.3), and for
+    // the other types, whose tiles of 64 have no deep buffers, also where they give every CU one cut along 512 (fp32 3000 x
+    // 1000 x 1000 39.7 against 43.7, 1000 x 1000 x 1000 29 against 22.7)
+    const bool small = tiles(128) < 192 && (type == NKMX_BF16 || tiles(128) * ((t + 511) / 512) <= 256);
+    p.side = tiles(256) * ((t + 1023) / 1024) >= 256 ? 256 : (small ? 64 : 128);
     const uint64_t bt = p.side == 256 && type != NKMX_BF16 ? 32 : 64;
     const uint64_t stages = (t + bt - 1) / bt, count = tiles(p.side);
     p.row_tiles = (n + p.side - 1) / p.side;
@@ -1874,7 +1938,26 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
             }
         }
     }
-    if (parts > stages / 8) parts = stages / 8;
+    if (p.side == 64) {
+        // A stage of a tile of 64 is mostly waiting, which two or three workgroups on a CU share (it takes 0.62, 0.9, 1.2 us, and
+        // 40 % more for each further one); against that stand 3 us for the join, 0.12 for each part's wait in it and the
+        // parts' bytes: 16384 x 300 x 500 bf16 (40 tiles) 12 parts 29.6, 24 30.8, 8 38; 1000 x 1000 x 1000 (256 tiles) whole
+        // 17.4, 3 parts 20.8; 1024 x 512 x 512 (64 tiles) whole 13.9, 4 parts 11.4.
+        const double stage = type == NKMX_BF16 ? 0.62 : type == NKMX_F16 ? 0.9 : 1.2;
+        const uint64_t resident = type == NKMX_F32 ? 2 : 3;
+        double best = 0;
+        parts = 1;
+        for (uint64_t q = 1; q == 1 || (q * count <= 256 * resident && q * 4 <= stages && q <= 64); ++q) {
+            const double us = (double)((stages + q - 1) / q) * stage * (1.0 + 0.4 * (double)((q * count - 1) / 256)) +
+                              (q > 1 ? 3.0 + (double)q * (0.12 + (double)n * (double)k * 1.2e-6) : 0.0);
+            if (q == 1 || us < best) {
+                best = us;
+                parts = q;
+            }
+        }
+    } else if (parts > stages / 8) {
+        parts = stages / 8;
+    }
     if (parts < 1) parts = 1;
     p.stages_each = (stages + parts - 1) / parts;
     p.parts = p.stages_each ? (stages + p.stages_each - 1) / p.stages_each : 1;

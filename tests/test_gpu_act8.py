@@ -377,3 +377,24 @@ def test_wgrad_of_a_few_tiles_more_than_cus(dtype):
     bound = (16 + parts * t / 16 + 257) * 2.0 ** -23 * (d64.abs() @ x64.abs())
     assert bool(((dw.double() - d64 @ x64).abs() <= bound).all())
     assert bool(((db.double() - d64.sum(1)).abs() <= (t / 4 + 16 + 257) * 2.0 ** -24 * d64.abs().sum(1)).all())
+
+
+@pytest.mark.parametrize("t,n,k", [(300, 1800, 2000), (2100, 64, 64), (700, 640, 650), (260, 70, 4100), (16384, 66, 130)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=name)
+def test_wgrad_of_contiguous_gradients(t, n, k, dtype):
+    """Tiles of 128 without a cut, of 64 with few and with many stages a part; the same bits again and without the bias."""
+    g = torch.Generator(device="cuda").manual_seed(t)
+    x = torch.randn(t, k, device="cuda", generator=g)
+    c, s = mx.act8_empty(t, k)
+    mx.cu_fn_act8_save_e(x, c, s)
+    mx.cu_fn_act8_load_e(x, c, s)
+    dy = torch.randn(t, n, device="cuda", generator=g).to(dtype)
+    dw, db = torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+    mx.cu_fn_act8_wgrad_e(dw, dy, c, s, DB=db)
+    d64 = f64(dy)
+    bound_w, bound_b = wgrad_bounds(d64, f64(x), t, dtype)
+    assert_within(dw, matmul64(d64.T, f64(x)), bound_w, "dw")
+    assert_within(db, d64.sum(0), bound_b, "db")
+    again = torch.empty_like(dw)
+    mx.cu_fn_act8_wgrad_e(again, dy, c, s)
+    assert torch.equal(again, dw)
