@@ -1967,6 +1967,8 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
     return p;
 }
 
+inline uint64_t workspace_of(const WgradPlan& p) { return p.parts > 1 ? p.parts * p.part_floats * 4 : 0; }
+
 template <typename T, int TN, int TK, int WN, int WK, int BT>
 inline int launch_wgrad(const WgradPlan& p, float* dw, uint64_t lddw, float* db, const T* dy, uint64_t lddy,
                         const uint8_t* codes, const uint8_t* scales, uint64_t t, uint64_t n, uint64_t k,
@@ -2192,8 +2194,7 @@ int nkmx_act8_grad(void* dx, const void* dy, int type, int fn, uint64_t rows, ui
 uint64_t nkmx_act8_wgrad_workspace(int type, uint64_t t, uint64_t n, uint64_t k)
 {
     if (!known_type(type) || t > kMaxSize || n > kMaxSize || k > kMaxSize || n == 0) return 0;
-    const WgradPlan p = wgrad_plan(type, t, n, k);
-    return p.parts > 1 ? p.parts * p.part_floats * 4 : 0;
+    return workspace_of(wgrad_plan(type, t, n, k));
 }
 
 int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, uint64_t n, uint64_t k, uint64_t lddw,
@@ -2206,7 +2207,8 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
     NKMX_TRY(check_packed(codes, scales, t, k));
     if (db && !on(db, 4)) return NKMX_EALIGN;
     if (n == 0 || (k == 0 && !db)) return NKMX_OK;
-    const uint64_t need = nkmx_act8_wgrad_workspace(type, t, n, k);
+    WgradPlan p = wgrad_plan(type, t, n, k);
+    const uint64_t need = workspace_of(p);
     if (need && (!workspace || workspace_bytes < need || !on(workspace, 16))) return NKMX_EWORK;
     const Area aw = area(dw, n, k, lddw, 4), ab = run(db, db ? n * 4 : 0), ad = area(dy, t, n, lddy, size_of(type));
     const Area ac = codes8(codes, t, k), as = scale_bytes(scales, t, k), ak = run(workspace, need);
@@ -2214,7 +2216,6 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
         if (overlap(*o, ad) || overlap(*o, ac) || overlap(*o, as)) return NKMX_EALIAS;
     if (overlap(aw, ab) || overlap(aw, ak) || overlap(ab, ak)) return NKMX_EALIAS;
     const hipStream_t s = (hipStream_t)stream;
-    WgradPlan p = wgrad_plan(type, t, n, k);
     if (p.col_tiles == 0) p.col_tiles = 1;  // k = 0: db alone
     const bool split = p.parts > 1;
     float* part = (float*)workspace;
