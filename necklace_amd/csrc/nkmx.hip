@@ -78,9 +78,9 @@ __device__ __forceinline__ float scale_value(uint32_t byte)
 // 2^(127 - byte) for bytes up to 253 (a finite number's byte is 252 at most).
 __device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// erfc(|x| / sqrt 2) / 2, the normal distribution's smaller side, by Abramowitz and Stegun's formula 7.1.26: erfc(z) =
-// (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), |error| <= 1.5e-7 (the factors 1 / sqrt 2 and 1 / 2 are in the
-// constants).  `tail` gets e^(-x^2 / 2).
+// gelu of the 16-bit types.  erfc(|x| / sqrt 2) / 2, the normal distribution's smaller side, by Abramowitz and Stegun's formula
+// 7.1.26: erfc(z) = (a1 t + .. + a5 t^5) e^(-z^2), t = 1 / (1 + p z), |error| <= 1.5e-7 (the factors 1 / sqrt 2 and 1 / 2 are in
+// the constants).  `tail` gets e^(-x^2 / 2).  Half a step of fp16 is 4.9e-4.
 __device__ __forceinline__ float smaller_side(float x, float& tail)
 {
     const float u = x * 0.84932180028801905f;  // u^2 = x^2 / (2 ln 2)
@@ -93,16 +93,61 @@ __device__ __forceinline__ float smaller_side(float x, float& tail)
     return p * t * tail;
 }
 
+// gelu of fp32, to a few roundings of the result.  Up to |x| = 1.25 (Phi(x) - 1/2) / x, and (Phi(x) - 1/2) / x + phi(x) for the
+// slope, are polynomials of x^2; beyond, the smaller side is e^(-x^2 / 2) t Q(t) with t = 1 / (1 + |x| / 4), which keeps its
+// digits as it vanishes.  The polynomials are least-maximum fits: off by 4e-9 and 1.5e-9 of 1/2, Q by 8e-9 of itself.  Relative
+// l2 error over normal inputs 3.1e-8 (slope 3.9e-8), where 0.5 x (1 + erf) in fp32 has 3.8e-8 (4.0e-8) and the formula above
+// 9e-8 (1.3e-7); 16384 x 4096 takes 93.8 us with it (slope 95.1), 91.6 (89.9) with the formula above.
+constexpr float kGeluBorder = 1.25f;
+template <int N>
+__device__ __forceinline__ float horner(const float (&c)[N], float x)
+{
+    float r = c[N - 1];
+#pragma unroll
+    for (int i = N - 2; i >= 0; --i) r = fmaf(r, x, c[i]);
+    return r;
+}
+// t Q(t); `tail` gets e^(-x^2 / 2).
+__device__ __forceinline__ float side_over_tail(float x, float& tail)
+{
+    constexpr float q[] = {0.0997423306f, 0.0995698348f, 0.0952199996f, 0.0711945295f,
+                           0.0975557268f, -0.0292390846f, 0.1140797958f, -0.0481649600f};
+    tail = __builtin_amdgcn_exp2f((x * x) * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.25f, 1.0f));
+    return horner(q, t) * t;
+}
+__device__ __forceinline__ float gelu32(float x)
+{
+    constexpr float p[] = {0.398942262f, -0.0664899871f, 0.00997150037f, -0.00118270959f, 0.000110327463f, -6.64486106e-6f};
+    const float u = x * x, near = fmaf(u, horner(p, u), 0.5f * x);
+    float tail;
+    const float side = side_over_tail(x, tail);
+    const float far = fmaf(-fabsf(x), side * tail, fmaxf(x, 0.0f));
+    return fabsf(x) < kGeluBorder ? near : far;
+}
+__device__ __forceinline__ float gelu32_slope(float x)
+{
+    constexpr float p[] = {0.797884524f, -0.265961289f, 0.0598397776f, -0.0094937738f, 0.00114656135f, -0.00010654654f, 6.19567072e-6f};
+    const float near = fmaf(x, horner(p, x * x), 0.5f);
+    float tail;
+    const float side = side_over_tail(x, tail);
+    const float w = tail * fmaf(fabsf(x), -0.39894228040143268f, side);
+    const float far = x < 0.0f ? w : 1.0f - w;
+    return fabsf(x) < kGeluBorder ? near : far;
+}
+
 __device__ __forceinline__ float logistic(float x)
 {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
-// fn(x) of a number.
-template <int FN>
+// fn(x) of a number of type T.
+template <int FN, typename T>
 __device__ __forceinline__ float activation(float x)
 {
-    if constexpr (FN == NKMX_GELU) {  // x Phi(x), without a choice by x's sign
+    if constexpr (FN == NKMX_GELU && std::is_same_v<T, float>) {
+        return gelu32(x);
+    } else if constexpr (FN == NKMX_GELU) {  // x Phi(x), without a choice by x's sign
         float tail;
         return fmaf(-fabsf(x), smaller_side(x, tail), fmaxf(x, 0.0f));
     } else if constexpr (FN == NKMX_SILU) {
@@ -111,18 +156,20 @@ __device__ __forceinline__ float activation(float x)
     return x;
 }
 // The same where x may be infinite or NaN: infinity stays, minus infinity times 0 is a NaN.
-template <int FN>
+template <int FN, typename T>
 __device__ __forceinline__ float activation_of_any(float x)
 {
-    const float y = activation<FN>(x);
+    const float y = activation<FN, T>(x);
     if (FN == NKMX_GELU && magnitude(x) >= kInfBits) return x > 0.0f ? x : __uint_as_float(0x7FC00000u);
     return y;
 }
 
-template <int FN>
+template <int FN, typename T>
 __device__ __forceinline__ float activation_slope(float x)
 {
-    if constexpr (FN == NKMX_GELU) {
+    if constexpr (FN == NKMX_GELU && std::is_same_v<T, float>) {
+        return gelu32_slope(x);
+    } else if constexpr (FN == NKMX_GELU) {
         float tail;
         const float side = smaller_side(x, tail);
         return fmaf(x * 0.39894228040143268f, tail, x < 0.0f ? side : 1.0f - side);
@@ -390,10 +437,10 @@ __global__ __launch_bounds__(256) void act8_save_kernel(const T* x, uint64_t ldx
         if constexpr (FN != NKMX_NONE) {
             typename Pack<T, E>::vec o;
 #pragma unroll
-            for (int i = 0; i < E; ++i) o[i] = (T)activation<FN>(number(v[u][i]));
+            for (int i = 0; i < E; ++i) o[i] = (T)activation<FN, T>(number(v[u][i]));
             if (byte == 255u) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) o[i] = (T)activation_of_any<FN>(number(v[u][i]));
+                for (int i = 0; i < E; ++i) o[i] = (T)activation_of_any<FN, T>(number(v[u][i]));
             }
             store_pack<T, E>(y + p[u].row * ldy + p[u].col, o, p[u].live);
         }
@@ -481,7 +528,7 @@ __global__ __launch_bounds__(256) void act8_grad_kernel(T* out, uint64_t ldo, co
             if constexpr (E == 8) four = code[u][i / 4];
             else four = code[u];
             const float v = (float)(int8_t)(four >> (8 * (i & 3))) * scale;
-            if constexpr (FN != NKMX_NONE) o[i] = (T)(number(g[u][i]) * activation_slope<FN>(v));
+            if constexpr (FN != NKMX_NONE) o[i] = (T)(number(g[u][i]) * activation_slope<FN, T>(v));
             else o[i] = (T)v;
         }
         store_pack<T, E>(out + p[u].row * ldo + p[u].col, o, p[u].live);
