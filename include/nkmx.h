@@ -86,9 +86,10 @@ uint64_t nkmx_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k);
 
 /*
  * x -> act8 codes of x, and y = fn(x) of the same type unless fn is NKMX_NONE (then y is NULL).  fn is
- * taken of x itself, not of its codes.  fp32 gelu and its slope are off by a few roundings of the
- * result, 16-bit gelu by a formula that is within 7.5e-7 of the normal distribution function, in fp32.
- * y may be x (with the same leading dimension).
+ * taken of x itself, not of its codes, in fp32.  For fp32 they and their slopes are off by a few
+ * roundings of the result (gelu, below -1.25: some 14 + 1.5 x^2 of them); for the 16-bit types gelu's
+ * formula is within 7.5e-7 of the normal distribution function.  y may be x (with the same leading
+ * dimension).
  */
 int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint64_t cols, uint64_t ldx, uint64_t ldy,
                    uint8_t* codes, uint8_t* scales, void* stream);

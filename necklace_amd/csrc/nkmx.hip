@@ -96,8 +96,8 @@ __device__ __forceinline__ float smaller_side(float x, float& tail)
 // gelu of fp32, to a few roundings of the result.  Up to |x| = 1.25 (Phi(x) - 1/2) / x, and (Phi(x) - 1/2) / x + phi(x) for the
 // slope, are polynomials of x^2; beyond, the smaller side is e^(-x^2 / 2) t Q(t) with t = 1 / (1 + |x| / 4), which keeps its
 // digits as it vanishes.  The polynomials are least-maximum fits: off by 4e-9 and 1.5e-9 of 1/2, Q by 8e-9 of itself.  Relative
-// l2 error over normal inputs 3.1e-8 (slope 3.9e-8), where 0.5 x (1 + erf) in fp32 has 3.8e-8 (4.0e-8) and the formula above
-// 9e-8 (1.3e-7); 16384 x 4096 takes 93.8 us with it (slope 95.1), 91.6 (89.9) with the formula above.
+// l2 error over normal inputs 2.8e-8 (slope 3.6e-8), where 0.5 x (1 + erf) in fp32 has 3.9e-8 (4.2e-8) and the formula above
+// 8.4e-8 (1.1e-7); 16384 x 4096 takes 93.8 us with it (slope 95.1), 91.6 (89.9) with the formula above.
 constexpr float kGeluBorder = 1.25f;
 template <int N>
 __device__ __forceinline__ float horner(const float (&c)[N], float x)
@@ -141,6 +141,38 @@ __device__ __forceinline__ float logistic(float x)
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
 
+// The logistic function of fp32 in two parts, g + g_low, and 1 - g in two parts, h + h_low.  With e = e^-|x| <= 1 nothing overflows:
+// they are 1 / (1 + e) and e / (1 + e), or the other way round.  What the exponential's argument, 1 + e, the reciprocal and
+// the product leave behind is carried in the lower parts: in fp32 alone the argument's rounding costs |x| / 2 units of e.  The
+// argument stops at 128, where e is 0.
+struct Logistic32 {
+    float g, g_low, h, h_low;
+};
+__device__ __forceinline__ Logistic32 logistic32(float x)
+{
+    const float a = fminf(fabsf(x), 128.0f), high = a * -1.44269502f;  // the upper and the lower part of -1 / ln 2
+    const float low = fmaf(a, -1.92596299e-8f, fmaf(a, -1.44269502f, -high));
+    const float e = __builtin_amdgcn_exp2f(high), e_low = e * 0.693147182f * low;
+    const float d = 1.0f + e, d_low = (e - (d - 1.0f)) + e_low;
+    const float q = __builtin_amdgcn_rcpf(d), q_low = fmaf(-q, d_low, fmaf(-q, d, 1.0f)) * q;
+    const float p = e * q, p_low = fmaf(e_low, q, fmaf(e, q_low, fmaf(e, q, -p)));
+    return x < 0.0f ? Logistic32{p, p_low, q, q_low} : Logistic32{q, q_low, p, p_low};
+}
+// x g.  Relative l2 error over normal inputs 2.6e-8, from -6 down 3.6e-8 (x / (1 + e^-x) in fp32 3.9e-8 and 3.5e-8, the form of
+// the 16-bit types 4.7e-8 and 2.1e-7); 16384 x 4096 91.4 us, as with that form.
+__device__ __forceinline__ float silu32(float x)
+{
+    const Logistic32 l = logistic32(x);
+    return fmaf(x, l.g, x * l.g_low);
+}
+// g (1 + x (1 - g)), 4.4e-8 and 5.9e-8 (4.8e-8 and 5.5e-8; 4.9e-8 and 1.8e-7); 92.3 us, 90.2 with that form.
+__device__ __forceinline__ float silu32_slope(float x)
+{
+    const Logistic32 l = logistic32(x);
+    const float s = fmaf(x, l.h_low, fmaf(x, l.h, 1.0f));
+    return fmaf(l.g, s, l.g_low * s);
+}
+
 // fn(x) of a number of type T.
 template <int FN, typename T>
 __device__ __forceinline__ float activation(float x)
@@ -150,6 +182,8 @@ __device__ __forceinline__ float activation(float x)
     } else if constexpr (FN == NKMX_GELU) {  // x Phi(x), without a choice by x's sign
         float tail;
         return fmaf(-fabsf(x), smaller_side(x, tail), fmaxf(x, 0.0f));
+    } else if constexpr (FN == NKMX_SILU && std::is_same_v<T, float>) {
+        return silu32(x);
     } else if constexpr (FN == NKMX_SILU) {
         return x * logistic(x);
     }
@@ -160,7 +194,7 @@ template <int FN, typename T>
 __device__ __forceinline__ float activation_of_any(float x)
 {
     const float y = activation<FN, T>(x);
-    if (FN == NKMX_GELU && magnitude(x) >= kInfBits) return x > 0.0f ? x : __uint_as_float(0x7FC00000u);
+    if ((FN == NKMX_GELU || std::is_same_v<T, float>) && magnitude(x) >= kInfBits) return x > 0.0f ? x : __uint_as_float(0x7FC00000u);
     return y;
 }
 
@@ -173,6 +207,8 @@ __device__ __forceinline__ float activation_slope(float x)
         float tail;
         const float side = smaller_side(x, tail);
         return fmaf(x * 0.39894228040143268f, tail, x < 0.0f ? side : 1.0f - side);
+    } else if constexpr (FN == NKMX_SILU && std::is_same_v<T, float>) {
+        return silu32_slope(x);
     } else if constexpr (FN == NKMX_SILU) {
         const float s = logistic(x);
         return s * fmaf(x, 1.0f - s, 1.0f);

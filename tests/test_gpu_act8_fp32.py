@@ -95,3 +95,29 @@ def test_large_numbers_and_infinities(fn):
         dx = torch.empty(1, 12, device="cuda")
         mx.cu_fn_act8_grad_e(dx, torch.ones_like(dx), c, s, fn)
         assert bool((dx == want).all())
+
+
+# silu.  x g with g = 1 / (1 + e) or e / (1 + e), e = e^-|x| off by the exponential's 2; sums, reciprocal and products are
+# carried in two parts, whose own roundings are 2^-24 of 2^-24; the last sum 1.  Below x = -87 e may be flushed.
+SILU_TINY = 2.0 ** -118
+
+
+@pytest.mark.parametrize("which", RANGES)
+def test_silu(which):
+    x = inputs(which)
+    c, s = mx.act8_empty(*x.shape)
+    y = torch.empty_like(x)
+    mx.cu_fn_act8_save_e(x, c, s, Y=y, fn="silu")
+    want = ref.activation(f64(x), "silu")
+    assert_within(y, want, 3.5 * HALF * np.abs(want) + SILU_TINY)
+
+
+# g (1 + x h) with g and h = 1 - g off by 2 as above, two roundings of the sum, one of the product.
+@pytest.mark.parametrize("which", RANGES)
+def test_silu_slope(which):
+    c, s, x = packed8(inputs(which))
+    dx = torch.empty(x.shape, device="cuda")
+    mx.cu_fn_act8_grad_e(dx, torch.full_like(dx, 2.0), c, s, "silu")
+    g, h = 1 / (1 + np.exp(-x)), 1 / (1 + np.exp(x))
+    want = g * (1 + x * h)
+    assert_within(dx, 2 * want, 2 * HALF * (5.5 * np.abs(want) + 2.5 * g * h * np.abs(x)) + SILU_TINY)
