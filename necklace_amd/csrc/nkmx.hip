@@ -1988,7 +1988,7 @@ struct WgradPlan {
     uint64_t part_floats;  // of dw and db of one part in the workspace
 };
 
-WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
+WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)  // n > 0
 {
     const auto tiles = [&](uint64_t side) { return ((n + side - 1) / side) * ((k + side - 1) / side); };
     WgradPlan p = {};
@@ -2000,11 +2000,12 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)
     const bool small = tiles(128) < 192 && (type == NKMX_BF16 || tiles(128) * ((t + 511) / 512) <= 256);
     p.side = tiles(256) * ((t + 1023) / 1024) >= 256 ? 256 : (small ? 64 : 128);
     const uint64_t bt = p.side == 256 && type != NKMX_BF16 ? 32 : 64;
-    const uint64_t stages = (t + bt - 1) / bt, count = tiles(p.side);
+    const uint64_t stages = (t + bt - 1) / bt;
     p.row_tiles = (n + p.side - 1) / p.side;
-    p.col_tiles = (k + p.side - 1) / p.side;
+    p.col_tiles = k ? (k + p.side - 1) / p.side : 1;  // k = 0: db alone, by one tile column
+    const uint64_t count = p.row_tiles * p.col_tiles;
     // split t until the tiles fill the chip, but keep 8 stages a part
-    uint64_t parts = count ? 256 / count : 1;
+    uint64_t parts = 256 / count;
     // More tiles than CUs: their last round may leave most CUs idle.  Cut in parts the rounds come out evenly, which is
     // weighed against writing and joining the parts: a tile of 256 takes 25, 50, 70 ns a token (bf16, fp16, fp32), a part
     // 1.8 ps a number (16384 x 4352 x 4096, 272 tiles: bf16 816 us whole, 645 in 3 parts, fp32 2322 and 1551 in 4; 16384 x
@@ -2290,7 +2291,7 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
     NKMX_TRY(check_packed(codes, scales, t, k));
     if (db && !on(db, 4)) return NKMX_EALIGN;
     if (n == 0 || (k == 0 && !db)) return NKMX_OK;
-    WgradPlan p = wgrad_plan(type, t, n, k);
+    const WgradPlan p = wgrad_plan(type, t, n, k);
     const uint64_t need = workspace_of(p);
     if (need && (!workspace || workspace_bytes < need || !on(workspace, 16))) return NKMX_EWORK;
     const Area aw = area(dw, n, k, lddw, 4), ab = run(db, db ? n * 4 : 0), ad = area(dy, t, n, lddy, size_of(type));
@@ -2299,7 +2300,6 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
         if (overlap(*o, ad) || overlap(*o, ac) || overlap(*o, as)) return NKMX_EALIAS;
     if (overlap(aw, ab) || overlap(aw, ak) || overlap(ab, ak)) return NKMX_EALIAS;
     const hipStream_t s = (hipStream_t)stream;
-    if (p.col_tiles == 0) p.col_tiles = 1;  // k = 0: db alone
     const bool split = p.parts > 1;
     float* part = (float*)workspace;
     float* to = split ? part : dw;
