@@ -1773,6 +1773,47 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_raw_ker
     }
 }
 
+// db alone (k = 0): sums of dy's columns.  A row of a tile is `lanes` lanes of 16 bytes, a power of two up to 64 that fits n, so
+// that narrow matrices still fill the wave with rows; a thread adds up every 256 / lanes-th row of its part of t, eight loads
+// on their way at a time, and the threads of a column are joined in order.  Bound by memory and by waits where few columns leave
+// few workgroups: with the join of the parts 16384 x 4096 bf16 (134 MB) 43 us, 16384 x 1023 50, 200000 x 64 26.
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_kernel(float* db, const T* dy, uint64_t lddy, uint32_t t_rows, uint32_t n,
+                                                          uint32_t lanes, uint32_t col_tiles, uint32_t rows_each,
+                                                          uint32_t accumulate, uint64_t part_stride)
+{
+    constexpr int E = Lanes<T>::E;
+    __shared__ float sums[256 * E];
+    const uint32_t groups = 256 / lanes, lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
+    const uint32_t tile = blockIdx.x % col_tiles, part = blockIdx.x / col_tiles;
+    const uint32_t first = part * rows_each, last = min(t_rows, first + rows_each);
+    const uint64_t col = ((uint64_t)tile * lanes + lane) * E;
+    const int64_t live = (int64_t)n - (int64_t)col;
+    float s[E] = {};
+    for (uint64_t t = first + group; t < last; t += 8 * groups) {
+        typename Pack<T, E>::vec v[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            v[i] = load_pack<T, E>(dy + (t + i * groups) * lddy + col, t + i * groups < last ? live : 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < E; ++j) s[j] += number(v[i][j]);
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) sums[threadIdx.x * E + j] = s[j];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < lanes * E; i += 256) {
+        float sum = sums[i];
+        for (uint32_t g = 1; g < groups; ++g) sum += sums[g * lanes * E + i];
+        const uint64_t c = (uint64_t)tile * lanes * E + i;
+        if (c < n) {
+            float* p = db + part * part_stride + c;
+            *p = accumulate ? *p + sum : sum;
+        }
+    }
+}
+
 // Joins the parts of a split weight gradient in order: dw, [parts][rows][ldp] in the workspace, and behind each part's
 // dw its db as a row of `rows` numbers.  Rows of the workspace are whole quads.  4 parts of 4096 x 1024 (84 MB) 12 .. 13
 // us = 6.5 TB/s.
@@ -1983,7 +2024,8 @@ int product(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint
 // ---- weight gradient
 
 struct WgradPlan {
-    int side;              // tile: 256, 128 or 64
+    int side;              // tile: 256, 128 or 64; 0: no columns, db alone, by tiles of `lanes` times 16 bytes of a row
+    uint32_t lanes;
     uint64_t row_tiles, col_tiles, parts, stages_each, ldp;
     uint64_t part_floats;  // of dw and db of one part in the workspace
 };
@@ -1992,6 +2034,20 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)  // n > 0
 {
     const auto tiles = [&](uint64_t side) { return ((n + side - 1) / side) * ((k + side - 1) / side); };
     WgradPlan p = {};
+    if (k == 0) {
+        // db alone: t is cut until there are two workgroups for every CU while a thread has 16 rows, in at most 64 parts, whose
+        // join waits 0.12 us for each
+        const uint64_t per_lane = 16 / size_of(type), wanted = (n + per_lane - 1) / per_lane;
+        p.lanes = 1;
+        while (p.lanes < 64 && p.lanes < wanted) p.lanes *= 2;
+        p.row_tiles = (wanted + p.lanes - 1) / p.lanes;
+        const uint64_t most = t / (256 / p.lanes * 16), fill = 512 / p.row_tiles;
+        p.parts = most < fill ? most : fill;
+        p.parts = p.parts < 1 ? 1 : p.parts > 64 ? 64 : p.parts;
+        p.stages_each = (t + p.parts - 1) / p.parts;
+        p.part_floats = (n + 3) / 4 * 4;
+        return p;
+    }
     // Tiles of 256 where they, cut along 1024 tokens, give every CU one (bf16, us with tiles of 256 / 128 / 64: 16384 x 1024
     // x 1024 56 / 70 / 88, 2048 x 4096 x 4096 74 / 94 / 152).  Else of 128 where nearly every CU has one without a cut (500 x
     // 2000 x 2000 bf16 20 against 25 with tiles of 64, fp32 27 against 33; 1000 x 1000 x 1000 bf16 23 against 16.3), and for
@@ -2002,7 +2058,7 @@ WgradPlan wgrad_plan(int type, uint64_t t, uint64_t n, uint64_t k)  // n > 0
     const uint64_t bt = p.side == 256 && type != NKMX_BF16 ? 32 : 64;
     const uint64_t stages = (t + bt - 1) / bt;
     p.row_tiles = (n + p.side - 1) / p.side;
-    p.col_tiles = k ? (k + p.side - 1) / p.side : 1;  // k = 0: db alone, by one tile column
+    p.col_tiles = (k + p.side - 1) / p.side;
     const uint64_t count = p.row_tiles * p.col_tiles;
     // split t until the tiles fill the chip, but keep 8 stages a part
     uint64_t parts = 256 / count;
@@ -2303,12 +2359,15 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
     const bool split = p.parts > 1;
     float* part = (float*)workspace;
     float* to = split ? part : dw;
-    float* to_db = !db ? nullptr : (split ? part + n * p.ldp : db);
+    float* to_db = !db ? nullptr : (split ? part + n * p.ldp : db);  // (ldp is 0 where there are no columns)
     const uint64_t ld = split ? p.ldp : lddw, stride = split ? p.part_floats : 0;
     const uint32_t add = !split && accumulate ? 1u : 0u;
     NKMX_TRY(for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
         constexpr int BT = Parts<T>::count == 1 ? 64 : 32;
+        if (p.side == 0)
+            return launch(column_sums_kernel<T>, dim3((uint32_t)(p.row_tiles * p.parts)), 256, s, to_db, (const T*)dy, lddy,
+                          (uint32_t)t, (uint32_t)n, p.lanes, (uint32_t)p.row_tiles, (uint32_t)p.stages_each, add, stride);
         if (p.side == 256)
             return launch_wgrad<T, 256, 256, 128, 64, BT>(p, to, ld, to_db, (const T*)dy, lddy, codes, scales, t, n, k, add,
                                                           stride, s);

@@ -56,11 +56,20 @@ def _save(x):
     return c, s
 
 
+def _column_sums(dy):
+    """fp32 sums of dy's columns: the weight gradient's bias alone.  (torch's sum clears its scratch memory by a graph node
+    that gives wrong sums when a captured graph is replayed.)"""
+    rows, n = mx.shape2(dy)
+    c, s = mx.act8_empty(rows, 0, device=dy.device)
+    db = torch.empty(n, dtype=torch.float32, device=dy.device)
+    mx.cu_fn_act8_wgrad_e(db.new_empty(n, 0), dy, c, s, DB=db, sync=False)
+    return db
+
+
 def _weight_grads(dy, c, s, weight_like, need_w, need_b):
     """Gradients of weight and bias from the checkpoint, in the weight's type."""
     if not need_w:
-        n = dy.shape[-1]
-        return None, (dy.reshape(-1, n).sum(0, dtype=torch.float32).to(dy.dtype) if need_b else None)
+        return None, (_column_sums(dy).to(dy.dtype) if need_b else None)
     n, k = weight_like
     dw = torch.empty(n, k, dtype=torch.float32, device=dy.device)
     db = torch.empty(n, dtype=torch.float32, device=dy.device) if need_b else None

@@ -9,10 +9,11 @@ TYPES = range(3)
 
 @pytest.mark.parametrize("ty", TYPES)
 def test_a_bias_gradient_alone_is_cut_as_its_workgroups_need(ty):
-    """k = 0: one workgroup for 64 columns of dy; parts only until they fill the chip (256 CUs, 3 workgroups each)."""
+    """k = 0: a workgroup for 64 lanes of 16 bytes of a row; parts only until there are two for each of 256 CUs."""
     need = _lib.mx_lib().nkmx_act8_wgrad_workspace
-    for n in (65536, 100000, 1 << 20):  # 1024 workgroups and more
+    width = 256 if ty == 0 else 512
+    for n in (width * 512, 1 << 20):
         assert need(ty, 16384, n, 0) == 0
-    for t, n in ((16384, 4096), (16384, 20000), (200000, 640), (5000, 30000)):
-        assert need(ty, t, n, 0) <= 768 // -(-n // 64) * (n + 3) * 4
-    assert need(ty, 64, 64, 0) == 0  # a single stage
+    for t, n in ((16384, 4096), (16384, 20000), (200000, 640), (5000, 30000), (2 ** 31 - 1, 64)):
+        assert need(ty, t, n, 0) <= min(64, 512 // -(-n // width)) * (n + 3) * 4
+    assert need(ty, 64, 64, 0) == 0
