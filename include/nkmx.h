@@ -89,7 +89,7 @@ uint64_t nkmx_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k);
  * taken of x itself, not of its codes, in fp32.  For fp32 they and their slopes are off by a few
  * roundings of the result (gelu, below -1.25: some 14 + 1.5 x^2 of them); for the 16-bit types gelu's
  * formula is within 7.5e-7 of the normal distribution function.  y may be x (with the same leading
- * dimension).
+ * dimension).  With an activation, codes and scales may both be NULL: y alone is written, the same bits.
  */
 int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint64_t cols, uint64_t ldx, uint64_t ldy,
                    uint8_t* codes, uint8_t* scales, void* stream);

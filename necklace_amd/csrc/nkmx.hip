@@ -468,8 +468,10 @@ __global__ __launch_bounds__(256) void act8_save_kernel(const T* x, uint64_t ldx
             w = low_bytes(q[0], q[1], q[2], q[3]);
             if (byte == 255u) w = 0u;
         }
-        reinterpret_cast<W*>(codes)[p[u].lane] = w;
-        store_scales<T>(scales, p[u], byte);
+        if (FN == NKMX_NONE || codes) {
+            reinterpret_cast<W*>(codes)[p[u].lane] = w;
+            store_scales<T>(scales, p[u], byte);
+        }
         if constexpr (FN != NKMX_NONE) {
             typename Pack<T, E>::vec o;
 #pragma unroll
@@ -2269,11 +2271,12 @@ int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint
     if (!known_type(type) || fn < NKMX_NONE || fn > NKMX_SILU) return NKMX_ERANGE;
     NKMX_TRY(check_matrix(x, type, rows, cols, ldx));
     if (fn != NKMX_NONE) NKMX_TRY(check_matrix(y, type, rows, cols, ldy));
-    NKMX_TRY(check_packed(codes, scales, rows, cols));
+    const bool saves = fn == NKMX_NONE || codes || scales;
+    if (saves) NKMX_TRY(check_packed(codes, scales, rows, cols));
     if (rows == 0 || cols == 0) return NKMX_OK;
     const uint64_t b = size_of(type);
     const Area ax = area(x, rows, cols, ldx, b), ay = area(y, fn == NKMX_NONE ? 0 : rows, cols, ldy, b);
-    const Area ac = codes8(codes, rows, cols), as = scale_bytes(scales, rows, cols);
+    const Area ac = codes8(codes, saves ? rows : 0, cols), as = scale_bytes(scales, saves ? rows : 0, cols);
     if (overlap(ac, ax) || overlap(as, ax) || overlap(ac, as) || overlap(ac, ay) || overlap(as, ay) ||
         (overlap(ay, ax) && !same(ay, ax)))
         return NKMX_EALIAS;

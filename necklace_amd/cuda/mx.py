@@ -303,10 +303,13 @@ def _fn_code(fn, none_allowed):
 
 def cu_fn_act8_save_e(A, C, S, Y=None, fn=None, stream=None, sync=True):
     """Checkpoint A in 8 bits (C, S from `act8_empty`) and, with `fn` ("gelu": x Phi(x), "silu": x / (1 + e^-x)), write
-    Y = fn(A) in the same pass, taken of A itself.  Y may be A."""
+    Y = fn(A) in the same pass, taken of A itself.  Y may be A.  With an activation, C and S may both be None: Y alone is
+    written, the same bits."""
     f = _fn_code(fn, True)
     rows, cols, ld = _matrix("A", A)
-    _packed("C", C, S, rows, cols, False, "A")
+    saves = fn is None or C is not None or S is not None
+    if saves:
+        _packed("C", C, S, rows, cols, False, "A")
     y, ldy = None, 0
     if fn is not None:
         yr, yc, ldy = _matrix("Y", Y)
@@ -319,8 +322,8 @@ def cu_fn_act8_save_e(A, C, S, Y=None, fn=None, stream=None, sync=True):
     dev = _device(A, C, S, Y)
     with _on_device(dev):
         h = nbutils.stream_handle(stream, dev)
-        code = _lib.mx_lib().nkmx_act8_save(A.data_ptr(), y, _TYPES[A.dtype], f, rows, cols, ld, ldy, C.data_ptr(),
-                                            S.data_ptr(), h)
+        code = _lib.mx_lib().nkmx_act8_save(A.data_ptr(), y, _TYPES[A.dtype], f, rows, cols, ld, ldy,
+                                            C.data_ptr() if saves else None, S.data_ptr() if saves else None, h)
         if code:
             _lib.check_mx(code)
         _finish(stream, dev, sync)

@@ -8,6 +8,8 @@ necklace_amd.cuda.mx.
                                    the rounding is treated as the identity (straight through)
     Mx4Weight(weight)              the codes alone, laid out once: .linear(x, bias) for serving
 
+Nothing is kept where no gradient can ask for it (without gradients enabled, or with inputs that need none).
+
 x is float32, bfloat16 or float16 on the GPU, [..., in]; weight [out, in] and bias [out] of the same type (autocast does
 not change them).  Gradients have their tensor's type; the weight gradient is summed in fp32 whatever that is.  The calls run on torch's current
 stream and can be captured into a graph.  A backward pass that is captured has to be the first use of its leaves'
@@ -79,8 +81,8 @@ def _weight_grads(dy, c, s, weight_like, need_w, need_b):
 
 class _Act8Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        ctx.saved_x = ctx.needs_input_grad[1]
+    def forward(ctx, x, weight, bias, keep):
+        ctx.saved_x = keep and ctx.needs_input_grad[1]
         ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
         with _as_given():
             return torch.nn.functional.linear(x, weight, bias)
@@ -94,15 +96,16 @@ class _Act8Linear(torch.autograd.Function):
             dx = dy @ weight if ctx.needs_input_grad[0] else None
         c, s = packed if ctx.saved_x else (None, None)
         dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
-        return dx, dw, db
+        return dx, dw, db, None
 
 
 class _Act8Act(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, fn):
+    def forward(ctx, x, fn, keep):
         x = _rows(x)
-        rows, cols = mx.shape2(x)
-        c, s = mx.act8_empty(rows, cols, device=x.device)
+        c = s = None
+        if keep and ctx.needs_input_grad[0]:
+            c, s = mx.act8_empty(*mx.shape2(x), device=x.device)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         mx.cu_fn_act8_save_e(x, c, s, Y=y, fn=fn, sync=False)
         ctx.save_for_backward(c, s)
@@ -116,13 +119,13 @@ class _Act8Act(torch.autograd.Function):
         dy = _rows(dy)
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
         mx.cu_fn_act8_grad_e(dx, dy, c, s, ctx.fn, sync=False)
-        return dx, None
+        return dx, None, None
 
 
 class _Mx4Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        ctx.saved_x = ctx.needs_input_grad[1]
+    def forward(ctx, x, weight, bias, keep):
+        ctx.saved_x = keep and ctx.needs_input_grad[1]
         ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
         return Mx4Weight(weight).linear(x, bias)
 
@@ -136,26 +139,26 @@ class _Mx4Linear(torch.autograd.Function):
             dx = Mx4Weight(weight, transpose=True).linear(dy)
         c, s = packed if ctx.saved_x else (None, None)
         dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
-        return dx, dw, db
+        return dx, dw, db, None
 
 
 def act8_linear(x, weight, bias=None):
     """torch.nn.functional.linear that keeps x in 8 bits (a quarter of fp32, half of 16 bits) for the weight gradient."""
     _check(x, weight, bias)
-    return _Act8Linear.apply(x, weight, bias)
+    return _Act8Linear.apply(x, weight, bias, torch.is_grad_enabled())
 
 
 def act8_act(x, fn):
     """fn(x) ("gelu": x Phi(x), "silu": x / (1 + e^-x)) that keeps x in 8 bits for its gradient."""
     _check(x)
     mx._fn_code(fn, False)
-    return _Act8Act.apply(x, fn)
+    return _Act8Act.apply(x, fn, torch.is_grad_enabled())
 
 
 def mx4_linear(x, weight, bias=None):
     """A linear layer whose products run on 4-bit operands, with gradients; the weight is laid out anew in every pass."""
     _check(x, weight, bias)
-    return _Mx4Linear.apply(x, weight, bias)
+    return _Mx4Linear.apply(x, weight, bias, torch.is_grad_enabled())
 
 
 class Mx4Weight:

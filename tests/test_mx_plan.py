@@ -17,3 +17,16 @@ def test_a_bias_gradient_alone_is_cut_as_its_workgroups_need(ty):
     for t, n in ((16384, 4096), (16384, 20000), (200000, 640), (5000, 30000), (2 ** 31 - 1, 64)):
         assert need(ty, t, n, 0) <= min(64, 512 // -(-n // width)) * (n + 3) * 4
     assert need(ty, 64, 64, 0) == 0
+
+
+FAR = 1 << 40
+
+
+def test_an_activation_without_its_checkpoint_is_named_by_two_null_pointers():
+    save = _lib.mx_lib().nkmx_act8_save
+    assert save(FAR, 2 * FAR, 0, 1, 0, 300, 300, 300, None, None, None) == 0
+    # past the check of the codes: y overlaps x
+    assert save(FAR, FAR + 4, 0, 1, 4, 300, 300, 300, None, None, None) == -4
+    assert save(FAR, 2 * FAR, 0, 1, 4, 300, 300, 300, 3 * FAR, None, None) == -1
+    assert save(FAR, 2 * FAR, 0, 1, 4, 300, 300, 300, None, 3 * FAR, None) == -1
+    assert save(FAR, None, 0, 0, 4, 300, 300, 300, None, None, None) == -1  # no activation: nothing to do but save
