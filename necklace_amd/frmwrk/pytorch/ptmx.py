@@ -10,9 +10,10 @@ necklace_amd.cuda.mx.
 
 Nothing is kept where no gradient can ask for it (without gradients enabled, or with inputs that need none).
 
-x is float32, bfloat16 or float16 on the GPU, [..., in]; weight [out, in] and bias [out] of the same type (autocast does
-not change them).  Gradients have their tensor's type; the weight gradient is summed in fp32 whatever that is.  The calls run on torch's current
-stream and can be captured into a graph.  A backward pass that is captured has to be the first use of its leaves'
+x is float32, bfloat16 or float16 on the GPU, [..., in]; weight [out, in] and bias [out] of the same type.  In an
+autocast region equal types stay as they are; different ones (bf16 activations beside fp32 weights) are cast to the region's
+type.  Gradients have their tensor's type; the weight gradient is summed in fp32 whatever that is.  The calls run on torch's
+current stream and can be captured into a graph.  A backward pass that is captured has to be the first use of its leaves'
 gradients on that stream (torch's own rule): take them with `torch.autograd.grad`, or let no eager graph of the same
 leaves live during the capture.  Second derivatives are not available.
 """
@@ -30,6 +31,17 @@ def _as_given():
 def _rows(t):
     """`t` where its strides are rows of neighbouring columns, else a contiguous copy (an expanded gradient)."""
     return t if mx.row_stride(t) is not None else t.contiguous()
+
+
+def _one_type(x, weight, bias):
+    """In an autocast region tensors of different types are cast to its type, as in torch's own linear layer; the casts
+    carry the gradients back to each tensor's own type."""
+    tensors = [x, weight] + ([] if bias is None else [bias])
+    if torch.is_autocast_enabled("cuda") and all(isinstance(t, torch.Tensor) and t.dtype in mx._TYPES for t in tensors) \
+            and any(t.dtype != x.dtype for t in tensors):
+        dtype = torch.get_autocast_dtype("cuda")
+        return tuple(t if t is None else t.to(dtype) for t in (x, weight, bias))
+    return x, weight, bias
 
 
 def _check(x, weight=None, bias=None):
@@ -144,6 +156,7 @@ class _Mx4Linear(torch.autograd.Function):
 
 def act8_linear(x, weight, bias=None):
     """torch.nn.functional.linear that keeps x in 8 bits (a quarter of fp32, half of 16 bits) for the weight gradient."""
+    x, weight, bias = _one_type(x, weight, bias)
     _check(x, weight, bias)
     return _Act8Linear.apply(x, weight, bias, torch.is_grad_enabled())
 
@@ -157,6 +170,7 @@ def act8_act(x, fn):
 
 def mx4_linear(x, weight, bias=None):
     """A linear layer whose products run on 4-bit operands, with gradients; the weight is laid out anew in every pass."""
+    x, weight, bias = _one_type(x, weight, bias)
     _check(x, weight, bias)
     return _Mx4Linear.apply(x, weight, bias, torch.is_grad_enabled())
 
@@ -177,6 +191,8 @@ class Mx4Weight:
             raise RuntimeError("Mx4Weight.linear has no gradient: use mx4_linear, or torch.no_grad()")
         if x.dim() < 1 or x.shape[-1] != self.shape[1]:
             raise ValueError(f"x {tuple(x.shape)} does not fit the weight {self.shape}")
+        if bias is not None and bias.dtype != x.dtype and torch.is_autocast_enabled("cuda"):
+            bias = bias.to(x.dtype)
         x = _rows(x)
         y = torch.empty(*x.shape[:-1], self.shape[0], dtype=x.dtype, device=x.device)
         mx.cu_fn_mx4_linear_e(y, x, self.codes, self.scales, bias=bias, sync=False)
