@@ -23,7 +23,9 @@
  *
  * Codes start on 16-byte boundaries, scales on 4-byte ones (NKMX_EALIGN otherwise); they are
  * contiguous.  Matrices of numbers have a leading dimension in elements (ld >= cols) and need the
- * alignment of their type only.  rows, cols, ld < 2^31.
+ * alignment of their type only.  rows, cols, ld < 2^31.  A product, weight gradient or transpose whose
+ * launch would take 2^32 threads (2^27 rows of a weight, 2^30 columns of a transpose, as orders of
+ * magnitude) gets NKMX_ERANGE; the passes along rows take all sizes.
  */
 #ifndef NKMX_H
 #define NKMX_H

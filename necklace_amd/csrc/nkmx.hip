@@ -317,7 +317,7 @@ struct Place {
 template <typename T, int U>
 __device__ __forceinline__ bool place_of(Place& p, int u, FastDiv steps, uint32_t n_steps, uint32_t cols)
 {
-    p.lane = (uint64_t)blockIdx.x * (256 * U) + (threadIdx.x >> 6) * (64 * U) + u * 64 + (threadIdx.x & 63);
+    p.lane = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 * U) + (threadIdx.x >> 6) * (64 * U) + u * 64 + (threadIdx.x & 63);
     const uint64_t step = p.lane / Lanes<T>::step;
     if (step >= n_steps) return false;  // all lanes of a step together
     p.row = quotient((uint32_t)step, steps);
@@ -1869,6 +1869,8 @@ inline void arg_pointers(Tuple& vals, void** out, std::index_sequence<I...>)
     ((out[I] = static_cast<void*>(&std::get<I>(vals))), ...);
 }
 
+constexpr uint64_t kMaxThreads = 1ull << 32;  // the runtime takes grids of fewer threads in a dimension
+
 template <typename... KArgs, typename... Args>
 inline int launch(void (*kernel)(KArgs...), dim3 grid, uint32_t block, hipStream_t s, Args... args)
 {
@@ -1943,6 +1945,14 @@ inline bool stream_of(Stream& s, uint64_t rows, uint64_t cols)
     return true;
 }
 
+// The grid of a streaming launch: one row of workgroups, or several where that would be too many threads (from 2^34 fp32 numbers on).
+inline dim3 stream_grid(const Stream& s)
+{
+    constexpr uint64_t most = kMaxThreads / 256 - 1;
+    const uint32_t y = (uint32_t)((s.blocks + most - 1) / most);
+    return dim3((s.blocks + y - 1) / y, y);
+}
+
 // The rules on matrices of numbers: sizes, leading dimension, alignment.
 inline int check_matrix(const void* p, int type, uint64_t rows, uint64_t cols, uint64_t ld)
 {
@@ -1983,7 +1993,8 @@ inline int launch_rows(T* y, uint64_t ldy, const T* x, uint64_t ldx, const uint8
                        hipStream_t s)
 {
     const uint64_t blocks = ((n + 16 * NT - 1) / (16 * NT)) * ((m + 16 * MT - 1) / (16 * MT));
-    if (blocks > kMaxSize) return NKMX_ERANGE;
+    if (blocks * (64 * kRowsWaves) >= kMaxThreads) return NKMX_ERANGE;
+    if (!y) return NKMX_OK;
     return launch(mx4_rows_kernel<T, MT, NT, FUSED>, dim3((uint32_t)blocks), 64 * kRowsWaves, s, y, ldy, x, ldx, ca, sa, cb, sb, bias,
                   (uint32_t)m, (uint32_t)n, (uint32_t)k, (uint32_t)steps_of(k));
 }
@@ -1993,7 +2004,8 @@ inline int launch_tiles(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa
                         const T* bias, uint64_t m, uint64_t n, uint64_t k, hipStream_t s)
 {
     const uint64_t rt = (m + TM - 1) / TM, ct = (n + TN - 1) / TN;
-    if (rt * ct > kMaxSize) return NKMX_ERANGE;
+    if (rt * ct * (64 * (TM / WM) * (TN / WN)) >= kMaxThreads) return NKMX_ERANGE;
+    if (!y) return NKMX_OK;
     return launch(mx4_tiles_kernel<T, TM, TN, WM, WN, BUFFERS>, dim3((uint32_t)(rt * ct)), 64 * (TM / WM) * (TN / WN), s, y, ldy,
                   ca, sa, cb, sb, bias, (uint32_t)m, (uint32_t)n, (uint32_t)steps_of(k), (uint32_t)rt, (uint32_t)ct);
 }
@@ -2007,6 +2019,7 @@ inline int launch_tiles(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa
 //                     12.6; with four buffers while every workgroup has a CU of its own (512 x 8192 x 8192 30 against 41
 //                     with two), with two beyond (2048 x 4096 x 4096 26.6 against 30.3)
 //   tiles 64 x 32     up to 128 tiles of 64: 64 x 8192 x 8192 15.0 against 17.2, but 128 x 8192 x 8192 21 against 17
+// Without y nothing is launched: whether the launch is one that the runtime takes.
 template <typename T>
 int product(T* y, uint64_t ldy, const uint8_t* ca, const uint8_t* sa, const uint8_t* cb, const uint8_t* sb,
             const T* bias, uint64_t m, uint64_t n, uint64_t k, hipStream_t s)
@@ -2117,7 +2130,7 @@ inline int launch_wgrad(const WgradPlan& p, float* dw, uint64_t lddw, float* db,
                         uint32_t accumulate, uint64_t stride, hipStream_t s)
 {
     const uint64_t tiles = p.row_tiles * p.col_tiles;
-    if (tiles > kMaxSize) return NKMX_ERANGE;
+    if (tiles * (64 * (TN / WN) * (TK / WK)) >= kMaxThreads) return NKMX_ERANGE;
     const auto with = [&](auto kernel) {
         return launch(kernel, dim3((uint32_t)tiles, (uint32_t)p.parts), 64 * (TN / WN) * (TK / WK), s, dw, lddw, db, dy, lddy,
                       codes, scales, (uint32_t)t, (uint32_t)n, (uint32_t)k, (uint32_t)steps_of(k), (uint32_t)p.row_tiles,
@@ -2169,7 +2182,7 @@ int nkmx_mx4_quantize(const void* x, int type, uint64_t rows, uint64_t cols, uin
             const auto with = [&](auto bytes) -> int {
                 constexpr int CPL = decltype(bytes)::value / (int)sizeof(T);
                 const uint64_t tiles = (cols + 64 * CPL - 1) / (64 * CPL), bands = (rows + 255) / 256;
-                if (tiles * bands > kMaxSize) return NKMX_ERANGE;
+                if (tiles * bands * 512 >= kMaxThreads) return NKMX_ERANGE;
                 return launch(mx4_quantize_transposed_kernel<T, CPL>, dim3((uint32_t)(tiles * bands)), 512, s, (const T*)x, ldx,
                               codes, scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)steps_of(rows), (uint32_t)tiles);
             };
@@ -2182,10 +2195,10 @@ int nkmx_mx4_quantize(const void* x, int type, uint64_t rows, uint64_t cols, uin
         // as they read lose by it)
         if (!stream_of<T, 4>(g, rows, cols)) return NKMX_ERANGE;
         if (g.blocks >= 1024)
-            return launch(mx4_quantize_kernel<T, 4>, dim3(g.blocks), 256, s, (const T*)x, ldx, codes, scales, g.steps,
+            return launch(mx4_quantize_kernel<T, 4>, stream_grid(g), 256, s, (const T*)x, ldx, codes, scales, g.steps,
                           g.n_steps, g.cols);
         stream_of<T, 1>(g, rows, cols);
-        return launch(mx4_quantize_kernel<T, 1>, dim3(g.blocks), 256, s, (const T*)x, ldx, codes, scales, g.steps, g.n_steps,
+        return launch(mx4_quantize_kernel<T, 1>, stream_grid(g), 256, s, (const T*)x, ldx, codes, scales, g.steps, g.n_steps,
                       g.cols);
     });
 }
@@ -2203,7 +2216,7 @@ int nkmx_mx4_dequantize(void* out, int type, uint64_t rows, uint64_t cols, uint6
         typedef std::remove_pointer_t<decltype(null)> T;
         Stream g;
         if (!stream_of<T, 1>(g, rows, cols)) return NKMX_ERANGE;
-        return launch(mx4_dequantize_kernel<T, 1>, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, codes, scales,
+        return launch(mx4_dequantize_kernel<T, 1>, stream_grid(g), 256, (hipStream_t)stream, (T*)out, ldo, codes, scales,
                       g.steps, g.n_steps, g.cols);
     });
 }
@@ -2255,7 +2268,10 @@ int nkmx_mx4_linear(void* y, const void* x, int type, uint64_t m, uint64_t n, ui
     const hipStream_t s = (hipStream_t)stream;
     uint8_t* ca = (uint8_t*)workspace;
     uint8_t* sa = ca + m * steps_of(k) * kStepBytes4;
-    if (need) NKMX_TRY(nkmx_mx4_quantize(x, type, m, k, ldx, ca, sa, 0, stream));
+    if (need) {
+        NKMX_TRY(product<float>(nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, m, n, k, s));
+        NKMX_TRY(nkmx_mx4_quantize(x, type, m, k, ldx, ca, sa, 0, stream));
+    }
     return for_type(type, [&](auto* null) -> int {
         typedef std::remove_pointer_t<decltype(null)> T;
         if (quantizes_inside(m, n, k))
@@ -2285,7 +2301,7 @@ int nkmx_act8_save(const void* x, void* y, int type, int fn, uint64_t rows, uint
         Stream g;
         if (!stream_of<T, 1>(g, rows, cols)) return NKMX_ERANGE;
         const auto with = [&](auto kernel) {
-            return launch(kernel, dim3(g.blocks), 256, (hipStream_t)stream, (const T*)x, ldx, (T*)y, ldy, codes, scales,
+            return launch(kernel, stream_grid(g), 256, (hipStream_t)stream, (const T*)x, ldx, (T*)y, ldy, codes, scales,
                           g.steps, g.n_steps, g.cols);
         };
         if (fn == NKMX_GELU) return with(act8_save_kernel<T, NKMX_GELU, 1>);
@@ -2311,7 +2327,7 @@ static int act8_read(void* out, const void* dy, int type, int fn, uint64_t rows,
         Stream g;
         if (!stream_of<T, 1>(g, rows, cols)) return NKMX_ERANGE;
         const auto with = [&](auto kernel) {
-            return launch(kernel, dim3(g.blocks), 256, (hipStream_t)stream, (T*)out, ldo, (const T*)dy, lddy, codes,
+            return launch(kernel, stream_grid(g), 256, (hipStream_t)stream, (T*)out, ldo, (const T*)dy, lddy, codes,
                           scales, g.steps, g.n_steps, g.cols);
         };
         if (fn == NKMX_GELU) return with(act8_grad_kernel<T, NKMX_GELU, 1>);
@@ -2360,6 +2376,8 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
     if (overlap(aw, ab) || overlap(aw, ak) || overlap(ab, ak)) return NKMX_EALIAS;
     const hipStream_t s = (hipStream_t)stream;
     const bool split = p.parts > 1;
+    const uint64_t join_blocks = (n * ((k + 3) / 4) + (db ? (n + 3) / 4 : 0) + 255) / 256;
+    if (split && join_blocks * 256 >= kMaxThreads) return NKMX_ERANGE;
     float* part = (float*)workspace;
     float* to = split ? part : dw;
     float* to_db = !db ? nullptr : (split ? part + n * p.ldp : db);  // (ldp is 0 where there are no columns)
@@ -2381,9 +2399,7 @@ int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, 
                                                    stride, s);
     }));
     if (!split) return NKMX_OK;
-    const uint64_t quads = n * ((k + 3) / 4) + (db ? (n + 3) / 4 : 0), blocks = (quads + 255) / 256;
-    if (blocks > kMaxSize) return NKMX_ERANGE;
-    return launch(join_parts_kernel, dim3((uint32_t)blocks), 256, s, dw, lddw, db, part, (uint32_t)p.parts, p.part_floats,
+    return launch(join_parts_kernel, dim3((uint32_t)join_blocks), 256, s, dw, lddw, db, part, (uint32_t)p.parts, p.part_floats,
                   (uint32_t)n, (uint32_t)k, p.ldp, accumulate ? 1u : 0u);
 }
 

@@ -30,3 +30,14 @@ def test_an_activation_without_its_checkpoint_is_named_by_two_null_pointers():
     assert save(FAR, 2 * FAR, 0, 1, 4, 300, 300, 300, 3 * FAR, None, None) == -1
     assert save(FAR, 2 * FAR, 0, 1, 4, 300, 300, 300, None, 3 * FAR, None) == -1
     assert save(FAR, None, 0, 0, 4, 300, 300, 300, None, None, None) == -1  # no activation: nothing to do but save
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """Sizes below 2^31 whose launch would take 2^32 threads: an argument error, before anything reaches a GPU."""
+    L, big = _lib.mx_lib(), 2 ** 31 - 1
+    matmul = lambda m, n, k: L.nkmx_mx4_matmul(FAR, 1, m, n, k, n, 2 * FAR, 3 * FAR, 4 * FAR, 5 * FAR, None, None)  # noqa: E731
+    assert matmul(1, big, 64) == -3 and matmul(16, 2 ** 28, 64) == -3 and matmul(big, 64, 64) == -3 and matmul(big, 1, 0) == -3
+    assert L.nkmx_mx4_quantize(FAR, 0, 1, big, big, 2 * FAR, 3 * FAR, 1, None) == -3
+    assert L.nkmx_mx4_linear(FAR, 2 * FAR, 1, 1, big, 1, big, 1, 3 * FAR, 4 * FAR, None, 5 * FAR, 1 << 20, None) == -3
+    for ty in TYPES:
+        assert L.nkmx_act8_wgrad(FAR, None, 2 * FAR, ty, 1, big, 1, 1, big, 3 * FAR, 4 * FAR, 0, None, 0, None) == -3
