@@ -44,19 +44,27 @@ def _one_type(x, weight, bias):
     return x, weight, bias
 
 
-def _check(x, weight=None, bias=None):
-    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
-        if t.dtype not in mx._TYPES or not t.is_cuda:
-            raise TypeError(f"{name}: expected a float32, bfloat16 or float16 GPU tensor, got {t.dtype} on {t.device}")
-        if t.dtype != x.dtype or t.device != x.device:
-            raise TypeError(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+def _check_tensor(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch tensor, got {type(t).__name__}")
+    if t.dtype not in mx._TYPES or not t.is_cuda:
+        raise TypeError(f"{name}: expected a float32, bfloat16 or float16 GPU tensor, got {t.dtype} on {t.device}")
+
+
+def _check(x, *weight_and_bias):
+    _check_tensor("x", x)
     if x.dim() < 1:
         raise ValueError("x: expected at least 1 dimension")
-    if weight is not None and (weight.dim() != 2 or weight.shape[1] != x.shape[-1]):
+    if not weight_and_bias:
+        return
+    weight, bias = weight_and_bias
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None and name == "bias":
+            continue
+        _check_tensor(name, t)
+        if t.dtype != x.dtype or t.device != x.device:
+            raise TypeError(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
         raise ValueError(f"weight {tuple(weight.shape)} does not fit x {tuple(x.shape)}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"bias {tuple(bias.shape)} does not fit weight {tuple(weight.shape)}")
@@ -179,6 +187,9 @@ class Mx4Weight:
     """The mx4 codes of a weight [out, in] (of its transpose with ``transpose=True``): 4.25 bits an element."""
 
     def __init__(self, weight, transpose=False):
+        _check_tensor("weight", weight)
+        if weight.dim() != 2:
+            raise ValueError(f"weight: expected 2 dimensions, got {weight.dim()}")
         w = _rows(weight.detach())
         n, k = w.shape
         self.shape = (k, n) if transpose else (n, k)
@@ -187,12 +198,19 @@ class Mx4Weight:
 
     def linear(self, x, bias=None):
         """mx4(x) W^T (+ bias), [..., in] -> [..., out]; for use without gradients."""
+        if not (isinstance(x, torch.Tensor) and x.is_cuda):
+            raise TypeError("x: expected a GPU tensor")
+        if bias is not None:
+            if not isinstance(bias, torch.Tensor):
+                raise TypeError(f"bias: expected a torch tensor, got {type(bias).__name__}")
+            if not bias.is_contiguous():
+                bias = bias.contiguous()
+            if bias.dtype != x.dtype and torch.is_autocast_enabled("cuda"):
+                bias = bias.to(x.dtype)
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError("Mx4Weight.linear has no gradient: use mx4_linear, or torch.no_grad()")
         if x.dim() < 1 or x.shape[-1] != self.shape[1]:
             raise ValueError(f"x {tuple(x.shape)} does not fit the weight {self.shape}")
-        if bias is not None and bias.dtype != x.dtype and torch.is_autocast_enabled("cuda"):
-            bias = bias.to(x.dtype)
         x = _rows(x)
         y = torch.empty(*x.shape[:-1], self.shape[0], dtype=x.dtype, device=x.device)
         mx.cu_fn_mx4_linear_e(y, x, self.codes, self.scales, bias=bias, sync=False)
