@@ -42,7 +42,7 @@ def test_bias_gradient_of_a_frozen_layer_in_a_graph(layer, t, n, dtype):
 
 
 @pytest.mark.parametrize("layer", [ptmx.act8_linear, ptmx.mx4_linear])
-@pytest.mark.parametrize("t,n,k", [(150, 60, 100), (20000, 64, 48), (3000, 1000, 520)])
+@pytest.mark.parametrize("t,n,k", [(150, 60, 100), (20000, 64, 48), (3000, 1000, 520), (32, 64, 8192), (32, 8192, 64), (1, 4096, 4096)])
 @pytest.mark.parametrize("dtype", DTYPES, ids=name)
 def test_a_layer_with_its_activation_in_a_graph(layer, t, n, k, dtype):
     """Result and all gradients of every replay against the eager calls, which run between the replays."""
@@ -103,3 +103,31 @@ def test_a_frozen_layer_without_outputs(layer):
     b = torch.randn(0, device="cuda", requires_grad=True)
     y = layer(x, w, b)
     assert torch.autograd.grad(y.sum(), b)[0].shape == (0,)
+
+
+@pytest.mark.parametrize("layer", [ptmx.act8_linear, ptmx.mx4_linear])
+def test_layers_on_another_stream(layer):
+    """Forward and backward behind slow work of a side stream: results and gradients as on the default one."""
+    x = values(1, 3000, 200, torch.bfloat16, 0.1)
+    w = values(2, 300, 200, torch.bfloat16, 0.1).requires_grad_()
+    b = torch.zeros(300, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    dy = values(3, 3000, 300, torch.bfloat16, 0.1)
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        y = ptmx.act8_act(layer(x, w, b), "silu")
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+
+    want = step(x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        late = torch.zeros_like(x)
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(10):
+            big = (big @ big).clamp(-1, 1)
+        late.copy_(x)
+        late += (big[0, 0] * 0).to(x.dtype)
+        got = step(late)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, e) for a, e in zip(got, want))
