@@ -152,27 +152,6 @@ def _device(first, *others):
     return dev
 
 
-class _Here:
-    """`with` nothing."""
-    __slots__ = ()
-
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        pass
-
-
-_HERE = _Here()
-# torch's accessor behind torch.cuda.current_device (0.06 us against 0.23); the documented route where it is absent
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
-def _on_device(index):
-    """`torch.cuda.device(index)` only when that is not the current one already."""
-    return _HERE if index == _current_device() else torch.cuda.device(index)
-
-
 @functools.lru_cache(maxsize=4096)
 def _linear_bytes(m, n, k):
     return int(_lib.mx_lib().nkmx_mx4_linear_workspace(m, n, k))
@@ -220,7 +199,7 @@ def cu_fn_mx4_quantize_e(A, C, S, transpose=False, stream=None, sync=True):
     pr, pc = (cols, rows) if transpose else (rows, cols)
     _packed("C", C, S, pr, pc, True, "A's transpose" if transpose else "A")
     dev = _device(A, C, S)
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         code = _lib.mx_lib().nkmx_mx4_quantize(A.data_ptr(), _TYPES[A.dtype], rows, cols, ld, C.data_ptr(), S.data_ptr(),
                                                1 if transpose else 0, h)
@@ -234,7 +213,7 @@ def cu_fn_mx4_dequantize_e(A, C, S, stream=None, sync=True):
     rows, cols, ld = _matrix("A", A)
     _packed("C", C, S, rows, cols, True, "A")
     dev = _device(A, C, S)
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         code = _lib.mx_lib().nkmx_mx4_dequantize(A.data_ptr(), _TYPES[A.dtype], rows, cols, ld, C.data_ptr(), S.data_ptr(), h)
         if code:
@@ -253,7 +232,7 @@ def cu_fn_mx4_matmul_e(Y, CA, SA, CB, SB, bias=None, stream=None, sync=True):
     _packed("CB", CB, SB, n, k, True, "Y and CA")
     b = _bias(bias, n, Y)
     dev = _device(Y, CA, SA, CB, SB, bias)
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         code = _lib.mx_lib().nkmx_mx4_matmul(Y.data_ptr(), _TYPES[Y.dtype], m, n, k, ld, CA.data_ptr(), SA.data_ptr(),
                                              CB.data_ptr(), SB.data_ptr(), b, h)
@@ -282,7 +261,7 @@ def cu_fn_mx4_linear_e(Y, X, CB, SB, bias=None, workspace=None, stream=None, syn
     b = _bias(bias, n, Y)
     dev = _device(Y, X, CB, SB, bias)
     L = _lib.mx_lib()
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         ws = _workspace(workspace, _linear_bytes(m, n, k), dev, stream, h)
         code = L.nkmx_mx4_linear(Y.data_ptr(), X.data_ptr(), _TYPES[Y.dtype], m, n, k, ldy, ldx, CB.data_ptr(),
@@ -320,7 +299,7 @@ def cu_fn_act8_save_e(A, C, S, Y=None, fn=None, stream=None, sync=True):
     elif Y is not None:
         raise ValueError("Y is written with an activation `fn` only")
     dev = _device(A, C, S, Y)
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         code = _lib.mx_lib().nkmx_act8_save(A.data_ptr(), y, _TYPES[A.dtype], f, rows, cols, ld, ldy,
                                             C.data_ptr() if saves else None, S.data_ptr() if saves else None, h)
@@ -334,7 +313,7 @@ def cu_fn_act8_load_e(A, C, S, stream=None, sync=True):
     rows, cols, ld = _matrix("A", A)
     _packed("C", C, S, rows, cols, False, "A")
     dev = _device(A, C, S)
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         code = _lib.mx_lib().nkmx_act8_load(A.data_ptr(), _TYPES[A.dtype], rows, cols, ld, C.data_ptr(), S.data_ptr(), h)
         if code:
@@ -352,7 +331,7 @@ def cu_fn_act8_grad_e(DX, DY, C, S, fn, stream=None, sync=True):
         raise ValueError(f"DY is {dr} x {dc}, DX {rows} x {cols}")
     _packed("C", C, S, rows, cols, False, "DX")
     dev = _device(DX, DY, C, S)
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         code = _lib.mx_lib().nkmx_act8_grad(DX.data_ptr(), DY.data_ptr(), _TYPES[DX.dtype], f, rows, cols, lddx, lddy,
                                             C.data_ptr(), S.data_ptr(), h)
@@ -388,7 +367,7 @@ def cu_fn_act8_wgrad_e(DW, DY, C, S, DB=None, accumulate=False, workspace=None, 
     dev = _device(DW, DY, C, S, DB)
     L = _lib.mx_lib()
     ty = _TYPES[DY.dtype]
-    with _on_device(dev):
+    with nbutils.on_device(dev):
         h = nbutils.stream_handle(stream, dev)
         ws = _workspace(workspace, _wgrad_bytes(ty, t, n, k), dev, stream, h)
         code = L.nkmx_act8_wgrad(DW.data_ptr(), db, DY.data_ptr(), ty, t, n, k, lddw, lddy, C.data_ptr(), S.data_ptr(),

@@ -57,3 +57,25 @@ def stream_handle(stream=None, device=None):
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+class _Here:
+    """`with` nothing."""
+    __slots__ = ()
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+# torch's accessor behind torch.cuda.current_device (0.06 us against 0.23); the documented route where it is absent
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def on_device(index):
+    """`with torch.cuda.device(index)` only when that is not the current device already: the libraries launch on the
+    current HIP device, and switching back and forth costs more than a small kernel takes."""
+    return _HERE if index == _current_device() else torch.cuda.device(index)

@@ -102,22 +102,8 @@ def _finish(stream, device, sync):
         stream.synchronize()
 
 
-class _on_device:
-    """`with torch.cuda.device(d)` only when d is not already the current device: the library launches
-    on the current HIP device, and switching back and forth costs more than a small kernel takes."""
-    __slots__ = ("ctx",)
-
-    def __init__(self, device):
-        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            return self.ctx.__exit__(*exc)
-        return False
+def _on_device(device):
+    return nbutils.on_device(device.index)
 
 
 _fn_cache = {}
