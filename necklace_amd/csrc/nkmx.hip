@@ -159,13 +159,13 @@ __device__ __forceinline__ Logistic32 logistic32(float x)
     return x < 0.0f ? Logistic32{p, p_low, q, q_low} : Logistic32{q, q_low, p, p_low};
 }
 // x g.  Relative l2 error over normal inputs 2.6e-8, from -6 down 3.6e-8 (x / (1 + e^-x) in fp32 3.9e-8 and 3.5e-8, the form of
-// the 16-bit types 4.7e-8 and 2.1e-7); 16384 x 4096 91.4 us, as with that form.
+// the 16-bit types 4.7e-8 and 2.1e-7).  16384 x 4096 91.4 us, as with that form; 1001 x 4097 from the caches 8.7 against 8.1.
 __device__ __forceinline__ float silu32(float x)
 {
     const Logistic32 l = logistic32(x);
     return fmaf(x, l.g, x * l.g_low);
 }
-// g (1 + x (1 - g)), 4.4e-8 and 5.9e-8 (4.8e-8 and 5.5e-8; 4.9e-8 and 1.8e-7); 92.3 us, 90.2 with that form.
+// g (1 + x (1 - g)), 4.4e-8 and 5.9e-8 (4.8e-8 and 5.5e-8; 4.9e-8 and 1.8e-7); 92.3 us against 90.2, 7.8 against 7.1.
 __device__ __forceinline__ float silu32_slope(float x)
 {
     const Logistic32 l = logistic32(x);
@@ -306,6 +306,10 @@ struct Lanes {
     static constexpr int row_blocks = 16 / block;      // blocks of a DPP row
 };
 
+// Workgroups of a row of the grid where a launch needs more than one (a constant: the grid's own size would be one more load
+// before the first address, 3.9 against 4.0 us for the quantise of 1001 x 4097 fp32).
+constexpr uint32_t kGridRow = 1u << 20;
+
 struct Place {
     uint64_t lane;     // index of the lane in the launch
     uint32_t row;
@@ -317,7 +321,7 @@ struct Place {
 template <typename T, int U>
 __device__ __forceinline__ bool place_of(Place& p, int u, FastDiv steps, uint32_t n_steps, uint32_t cols)
 {
-    p.lane = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 * U) + (threadIdx.x >> 6) * (64 * U) + u * 64 + (threadIdx.x & 63);
+    p.lane = ((uint64_t)blockIdx.y * kGridRow + blockIdx.x) * (256 * U) + (threadIdx.x >> 6) * (64 * U) + u * 64 + (threadIdx.x & 63);
     const uint64_t step = p.lane / Lanes<T>::step;
     if (step >= n_steps) return false;  // all lanes of a step together
     p.row = quotient((uint32_t)step, steps);
@@ -576,8 +580,9 @@ __global__ __launch_bounds__(256) void act8_grad_kernel(T* out, uint64_t ldo, co
 // The transpose: blocks run down x's columns.  A workgroup of 8 waves takes 256 rows x 64 * CPL columns; a wave
 // takes 32 rows = one block of every column, a lane CPL columns (one load of 4 or 8 bytes a row), so a block
 // never leaves its lane.  The codes cross LDS once, so that a column's 256 rows leave as 128
-// contiguous bytes: whole cache lines.  Bound by memory: 8192 x 4096 fp32 (152 MB) 25.8 us = 5.9 TB/s; rows off the cache
-// lines, which neighbouring tiles then share, 8191 x 4097 30 us = 5.1 TB/s.
+// contiguous bytes: whole cache lines.  Bound by memory and by rounds of workgroups that load once and store once, three on a
+// CU: 8192 x 4096 fp32 (152 MB, 1024 of them) 26.8 us = 5.7 TB/s.  A further tile column leaves some CUs two in the last round:
+// 8192 x 4160 29.1, 8192 x 4224 29.6; with rows off the cache lines, which neighbours then share (5 % more bytes), 8191 x 4097 30.4.
 template <typename T, int CPL>
 __global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x, uint64_t ldx, uint8_t* codes,
                                                                       uint8_t* scales, uint32_t rows, uint32_t cols,
@@ -1948,9 +1953,8 @@ inline bool stream_of(Stream& s, uint64_t rows, uint64_t cols)
 // The grid of a streaming launch: one row of workgroups, or several where that would be too many threads (from 2^34 fp32 numbers on).
 inline dim3 stream_grid(const Stream& s)
 {
-    constexpr uint64_t most = kMaxThreads / 256 - 1;
-    const uint32_t y = (uint32_t)((s.blocks + most - 1) / most);
-    return dim3((s.blocks + y - 1) / y, y);
+    if ((uint64_t)s.blocks * 256 < kMaxThreads) return dim3(s.blocks);
+    return dim3(kGridRow, (s.blocks - 1) / kGridRow + 1);
 }
 
 // The rules on matrices of numbers: sizes, leading dimension, alignment.
