@@ -99,23 +99,34 @@ def _weight_grads(dy, c, s, weight_like, need_w, need_b):
     return dw.to(dy.dtype), db.to(dy.dtype) if need_b else None
 
 
+def _keep(ctx, x, weight, keep):
+    """What backward reads: the weight for the input's gradient, the checkpoint of x for the weight's."""
+    ctx.weight_shape = weight.shape
+    ctx.saved_w, ctx.saved_x = keep and ctx.needs_input_grad[0], keep and ctx.needs_input_grad[1]
+    ctx.save_for_backward(*((weight,) if ctx.saved_w else ()), *(_save(x) if ctx.saved_x else ()))
+
+
+def _kept(ctx):
+    """(weight, codes, scales), None where not kept."""
+    kept = ctx.saved_tensors
+    return (kept[0] if ctx.saved_w else None,) + (kept[-2:] if ctx.saved_x else (None, None))
+
+
 class _Act8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, keep):
-        ctx.saved_x = keep and ctx.needs_input_grad[1]
-        ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
+        _keep(ctx, x, weight, keep)
         with _as_given():
             return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        weight, *packed = ctx.saved_tensors
+        weight, c, s = _kept(ctx)
         dy = _rows(dy)
         with _as_given():
             dx = dy @ weight if ctx.needs_input_grad[0] else None
-        c, s = packed if ctx.saved_x else (None, None)
-        dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        dw, db = _weight_grads(dy, c, s, ctx.weight_shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return dx, dw, db, None
 
 
@@ -145,20 +156,18 @@ class _Act8Act(torch.autograd.Function):
 class _Mx4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, keep):
-        ctx.saved_x = keep and ctx.needs_input_grad[1]
-        ctx.save_for_backward(weight, *(_save(x) if ctx.saved_x else ()))
+        _keep(ctx, x, weight, keep)
         return Mx4Weight(weight).linear(x, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        weight, *packed = ctx.saved_tensors
+        weight, c, s = _kept(ctx)
         dy = _rows(dy)
         dx = None
         if ctx.needs_input_grad[0]:
             dx = Mx4Weight(weight, transpose=True).linear(dy)
-        c, s = packed if ctx.saved_x else (None, None)
-        dw, db = _weight_grads(dy, c, s, weight.shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        dw, db = _weight_grads(dy, c, s, ctx.weight_shape, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return dx, dw, db, None
 
 

@@ -81,3 +81,22 @@ def test_half_a_checkpoint_is_refused():
             mx.cu_fn_act8_save_e(x, *pair, Y=torch.empty_like(x), fn="gelu")
     with pytest.raises(TypeError, match="torch tensor"):
         mx.cu_fn_act8_save_e(x, None, None)
+
+
+@pytest.mark.parametrize("layer", [ptmx.act8_linear, ptmx.mx4_linear])
+def test_a_weight_that_no_gradient_reads_may_change(layer):
+    """Only the input's gradient reads the weight: without it the weight may be updated before the backward pass, as with
+    torch's linear layer; with it the change is noticed."""
+    x, w = values(1, 50, 100, torch.float32), values(2, 30, 100, torch.float32).requires_grad_()
+    dy = values(3, 50, 30, torch.float32)
+    want, = torch.autograd.grad(layer(x, w), w, dy)
+    y = layer(x, w)
+    with torch.no_grad():
+        w.add_(1)
+    got, = torch.autograd.grad(y, w, dy)
+    assert torch.equal(got, want)
+    y = layer(x.requires_grad_(), w)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(y, (x, w), dy)
