@@ -655,7 +655,7 @@ __global__ __launch_bounds__(512) void mx4_quantize_transposed_kernel(const T* x
 // are joined through LDS in wave order.  FUSED: a lane quantizes its own block of 32 numbers of x in registers, with the
 // arithmetic of mx4_quantize_kernel.
 //
-// Rows of a x n x k, codes from HBM: 1 x 4096 x 1024 2.7 us (its 2.2 MB are 0.3): a launch and three memory latencies in a
+// Rows of a x n x k, codes from HBM: 1 x 4096 x 1024 3.1 us (its 2.2 MB are 0.3): a launch and three memory latencies in a
 // chain; 1 x 8192 x 8192 (36 MB) 9.6; 1 x 28672 x 8192 (125 MB) 26.3 = 4.7 TB/s, 1 x 65536 x 4096 (143 MB) 26 = 5.5 TB/s,
 // 16 x 28672 x 8192 36: a's rows from L2 are as many bytes as b's then.  Loads of whole lines of 8 rows for two
 // instructions each gained nothing over this; k split over 4, 2 or 1 of the waves is slower from k = 4096 on (1 x 8192 x
@@ -847,7 +847,7 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t row_tiles, uint32_t
 // load writes LDS in lane order, so the lanes' addresses carry the exchange.  The buffer's extent ends the rows: a
 // row past the matrix is not read, and its results are not stored.
 //
-// 8192 x 8192 x 8192: 261 .. 275 us = 4.0 .. 4.2 PFLOP/s in a row of calls, 281 .. 294 between other work; the instructions
+// 8192 x 8192 x 8192: 276 .. 283 us = 3.9 .. 4.0 PFLOP/s in a row of calls, 283 .. 293 between other work; the instructions
 // alone would take 139.  The same launch on codes of zeros takes 202: half of what is left is the clock, which falls
 // with the power that random operands take.  The rest is LDS, where a wave of 128 x 64 reads 6 operands for 8
 // instructions, and the wait at the one barrier of a stage.  Waves of 128 x 128 read a third less and take 267 .. 290 (one a
@@ -1119,7 +1119,8 @@ __global__ __launch_bounds__(64 * (TM / WM) * (TN / WN)) void mx4_tiles_kernel(
 // blockIdx.y where there are few tiles; the parts are joined in order by a second kernel.
 //
 // Bound by the matrix instructions and the LDS traffic and turning between them: fp32 16384 x 4352 x 4096 1551 us, 1.13
-// PFLOP/s of bf16 products; 5001 x 1023 x 4097 (3 parts of 68 tiles: 204 of 256 CUs) 138 us and 11 to join.
+// PFLOP/s of bf16 products; 5001 x 1023 x 4097 (3 parts of 68 tiles: 204 of 256 CUs) 135 us with the join in a row of calls, 136
+// and 12 as single launches.
 
 template <int SLOTS>
 __device__ __forceinline__ uint32_t swizzle_t(uint32_t c)
@@ -1476,9 +1477,10 @@ __global__ __launch_bounds__(64 * (TN / WN) * (TK / WK)) void act8_wgrad_kernel(
 // instructions cover the first reads of the next stage.  Tiles of 64 have one instruction for each 16 tokens and are bound
 // by waiting: they read a stage's operands at once and ask for dy three stages ahead (0.62 us a stage against 0.86).
 //
-// 16384 x 4096 x 4096: 472 us = 1.16 PFLOP/s, where a large bf16 library product runs at 1.20 to 1.35; 16384 x 4096 x 1024 (4
-// parts of 64 tiles) 138 us, of which the parts' stores are some 15, and 14 to join; the kernel above takes 177 and 14.  On
-// zeros both calls take a fifth less (376, and 122 with the join): the clock falls with the power of random operands, as for
+// 16384 x 4096 x 4096: 482 us = 1.14 PFLOP/s, where a large bf16 library product runs at 1.20 to 1.35; 16384 x 4096 x 1024 (4
+// parts of 64 tiles) 149 us with the join, of which the parts' stores are some 15 and the join 14; with the kernel above 198
+// (16384 x 4096 x 4096 673).  On
+// zeros both calls take a fifth to an eighth less (390, and 130 with the join): the clock falls with the power of random operands, as for
 // the library.  Waves of 64 x 128, late waves, wave priorities, other orders of the tiles and a touch of L2 two stages
 // ahead were no faster.
 template <int TN, int TK, int WN, int WK>
