@@ -108,8 +108,9 @@ int nkmx_act8_grad(void* dx, const void* dy, int type, int fn, uint64_t rows, ui
  * dw[j, c] = (accumulate ? dw[j, c] : 0) + sum over i of dy[i, j] * x^[i, c] for dy [t, n] of `type` and x
  * [t, k] in act8; dw is fp32 [n, k].  db (fp32 [n], may be NULL) gets the sums of dy's columns the same
  * way.  Every product is exact and the sums are fp32 for all three types (an fp32 dy keeps all its bits
- * from 2^-110 up).  The result does not depend on timing.  `workspace`: nkmx_act8_wgrad_workspace
- * bytes on a 16-byte boundary, NULL if that is 0.
+ * from 2^-110 up).  k = 0 gives db alone (dw, codes and scales are not read or written).  The result does
+ * not depend on timing.  `workspace`: nkmx_act8_wgrad_workspace bytes on a 16-byte boundary, NULL if that
+ * is 0.
  */
 int nkmx_act8_wgrad(float* dw, float* db, const void* dy, int type, uint64_t t, uint64_t n, uint64_t k, uint64_t lddw,
                     uint64_t lddy, const uint8_t* codes, const uint8_t* scales, int accumulate, void* workspace,

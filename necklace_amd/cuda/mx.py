@@ -348,8 +348,9 @@ def act8_wgrad_workspace(dtype, t, n, k):
 def cu_fn_act8_wgrad_e(DW, DY, C, S, DB=None, accumulate=False, workspace=None, stream=None, sync=True):
     """Weight gradient of a linear layer from the checkpoint of its input: DW[j, c] = sum over i of DY[i, j] x[i, c],
     x [t, k] given by C, S.  DW is float32 [n, k], DY [t, n] of any of the types; DB (float32 [n]) gets the sums of DY's
-    columns.  ``accumulate=True`` adds to what DW and DB hold.  Products are exact and sums fp32 for every type; the
-    result is the same bits every time.  `workspace` as in `cu_fn_mx4_linear_e`, of `act8_wgrad_workspace` bytes."""
+    columns (alone, where k is 0).  ``accumulate=True`` adds to what DW and DB hold.  Products are exact and sums fp32 for
+    every type; the result is the same bits every time.  `workspace` as in `cu_fn_mx4_linear_e`, of `act8_wgrad_workspace`
+    bytes."""
     n, k, lddw = _matrix("DW", DW)
     if DW.dtype != torch.float32:
         raise TypeError(f"DW: expected float32, got {DW.dtype}")
